@@ -87,6 +87,12 @@ int rbn_device_count(void);
 /* Creates a context on `device`.  Replaces BitNetExecutionProvider::with_config's
  * resource set-up (provider.rs:77-114). */
 int rbn_ctx_create(int device, rbn_ctx **out);
+/* The same on a stream of the caller's (a hipStream_t; NULL is the device's default stream):
+ * every call of the context is ordered with what the caller queues there itself, so memory that
+ * another library fills on that stream needs no synchronisation in between.  The stream must
+ * belong to `device` and outlive the context, which never destroys it.  Graph capture
+ * needs a stream that HIP can capture (not the default one).  No reference counterpart. */
+int rbn_ctx_create_on_stream(int device, void *stream, rbn_ctx **out);
 int rbn_ctx_destroy(rbn_ctx *ctx);
 int rbn_get_device_info(rbn_ctx *ctx, rbn_device_info *out);
 
@@ -103,6 +109,9 @@ int rbn_sync(rbn_ctx *ctx);
  * context: *h_flags receives the bits raised since the last call and the word is cleared.
  * Synchronises the stream.  No reference counterpart. */
 #define RBN_FLAG_HISTORY_OVERFLOW 1u /* rbn_argmax_f32 / rbn_greedy_next_f32: position outside the history */
+#define RBN_FLAG_KV_REFUSED 2u       /* rbn_kv_plan: a row got no tokens (no page left, row or batch full) */
+#define RBN_FLAG_KV_BAD_INDEX 4u     /* a row, position, length or page outside its range: that item was left out */
+#define RBN_FLAG_KV_NONFINITE 8u     /* rbn_rope_kv_store_q8: a NaN became 0 or a value beyond f16 was saturated */
 int rbn_device_flags(rbn_ctx *ctx, uint32_t *h_flags);
 /* Bytes currently / at most allocated through rbn_malloc on this context
  * (MemoryInfo, allocator.rs:142-148). */
@@ -349,6 +358,115 @@ int rbn_argmax_f32(rbn_ctx *ctx, const float *d_values, uint64_t n, int32_t *d_i
 int rbn_greedy_next_f32(rbn_ctx *ctx, const float *d_logits, uint64_t vocab, int32_t *d_token,
                         int32_t *d_history, int32_t *d_pos, uint64_t history_capacity,
                         const float *d_table, uint64_t H, float *d_x);
+/* Log probabilities of given tokens: for each of `rows` rows of `vocab` f32 logits (row r at
+ * d_logits + r * pitch, pitch >= vocab), with lse = log sum_i exp(x_i),
+ *   d_logprob[r]  = x[d_target[r]] - lse         (a target outside [0, vocab): 0)
+ *   d_entropy[r]  = -sum_i p_i log p_i, p_i = exp(x_i - lse)   (a term with p_i = 0 is 0)
+ *   d_top_token[r, j], d_top_logprob[r, j], j < top: the largest logits in descending order, the
+ *     lowest index first among equals, and x - lse; entries past the vocabulary are -1 and -inf.
+ * -inf is an ordinary masked logit; a row of nothing else has log probabilities of -inf and
+ * entropy 0.  A NaN or +inf makes the row's log probabilities and its entropy NaN; a NaN ranks
+ * below every number.  top <= RBN_TOP_MAX; d_logprob (with d_target), d_entropy and the two top
+ * arrays are each optional (NULL; top = 0).  One pass over the logits. */
+#define RBN_TOP_MAX 32
+int rbn_token_logprobs_f32(rbn_ctx *ctx, const float *d_logits, uint64_t rows, uint64_t vocab,
+                           uint64_t pitch, const int32_t *d_target, uint64_t top, float *d_logprob,
+                           float *d_entropy, int32_t *d_top_token, float *d_top_logprob);
+
+/* ---- serving several sequences: paged 8-bit K/V cache (no reference counterpart) ----- */
+/* A ROW is the place of one sequence in a batch.  Its positions are cut into blocks of
+ * RBN_KV_BLOCK; a full block lives in a PAGE (one page number for all layers and K/V heads),
+ * in 8 bits with one f32 scale for each (page, K/V head) of K and of V; the row's last, unfinished
+ * block lives in f16 in the row's "open" buffer of each layer.  What the cache holds for a sequence
+ * therefore does not depend on how its tokens were split into calls:
+ *   x = f16(k) of every token (rotated k; v as it is); values beyond f16 are saturated, NaN becomes
+ *   0, either raises RBN_FLAG_KV_NONFINITE;
+ *   full block: scale = max|x| / 127 (RBN_KV_I8) or / 448 (RBN_KV_E4M3), code = round to nearest even
+ *   of x / scale to int8 or e4m3; the cache holds code * scale (0 where the scale is 0).
+ * The descriptors below are HOST structs of device pointers; they are copied into the launches,
+ * so they may be reused as soon as a call returns and every call can be captured in a graph
+ * (the numbers of rows and tokens may differ from replay to replay: the kernels read them from device
+ * memory).  Numbers out of range in device memory never lead outside the buffers: the item is left
+ * out and RBN_FLAG_KV_BAD_INDEX raised.  Which rows, pages and calls belong together is the caller's
+ * affair: a page handed out twice, or two rows of d_table sharing a page that one of them
+ * still fills, gives wrong values. */
+#define RBN_KV_BLOCK 32
+#define RBN_KV_MAX_ROWS 2048
+#define RBN_KV_MAX_BLOCKS (1u << 20)  /* of one row */
+#define RBN_KV_MAX_TOKENS (1u << 18)  /* of one call */
+typedef enum rbn_kv_format { RBN_KV_I8 = 0, RBN_KV_E4M3 = 1 } rbn_kv_format;
+typedef struct rbn_kv_table {
+    uint64_t rows;               /* 1 to RBN_KV_MAX_ROWS */
+    uint64_t max_blocks;         /* blocks a row may have, 1 to RBN_KV_MAX_BLOCKS */
+    uint64_t pages;              /* pages of the pool, 1 to 2^31 / RBN_KV_BLOCK - 1 */
+    int32_t *d_table;            /* [rows, max_blocks] page of each block */
+    const int32_t *d_len;        /* [rows] positions held */
+    int32_t *d_ring;             /* [pages] free pages, a ring: taken at the head, returned behind the tail */
+    const int32_t *d_ring_state; /* [2] head, number of free pages */
+} rbn_kv_table;
+typedef struct rbn_kv_batch {
+    uint64_t max_tokens;         /* capacity of the arrays below, 1 to RBN_KV_MAX_TOKENS */
+    int32_t *d_start;            /* [rows + 1] first token of each row; [rows] = tokens in all */
+    int32_t *d_row;              /* [max_tokens] row of each token */
+    int32_t *d_pos;              /* [max_tokens] position in its row */
+    int32_t *d_slot;             /* [max_tokens] page * RBN_KV_BLOCK + position % RBN_KV_BLOCK */
+    int32_t *d_unit;             /* [max_tokens] first token of each (row, block) the call touches */
+    int32_t *d_count;            /* [2] tokens, units */
+} rbn_kv_batch;
+typedef struct rbn_kv_layer {
+    uint32_t format;             /* rbn_kv_format */
+    uint32_t kv_heads;           /* 1 to 1024 */
+    uint32_t head_dim;           /* 64 or 128 */
+    uint32_t reserved;           /* set to 0 */
+    void *d_k;                   /* [pages, kv_heads, RBN_KV_BLOCK * head_dim] codes, 16-byte aligned like the three below; inside
+                                  * a page head, code (t, d) of K is at byte
+                                  * ((t/16 * (head_dim/64) + d/64) * 64 + d%32/8 * 16 + t%16) * 16 + d/32%2 * 8 + d%8 */
+    void *d_v;                   /* ... and code (t, d) of V at byte
+                                  * (d/32 * 64 + t%16/4 * 16 + d%16) * 16 + d/16%2 * 8 + t/16 * 4 + t%4 */
+    void *d_k_open;              /* [rows, kv_heads, RBN_KV_BLOCK, head_dim] f16 */
+    void *d_v_open;
+    float *d_k_scale;            /* [pages, kv_heads] */
+    float *d_v_scale;
+} rbn_kv_layer;
+/* Bytes of one layer's buffers: codes of K (or V), scales of K (or V), open blocks of K (or V); 0 for
+ * arguments outside the ranges above.  Needs no device. */
+size_t rbn_kv_code_bytes(uint64_t pages, uint64_t kv_heads, uint64_t head_dim);
+size_t rbn_kv_scale_bytes(uint64_t pages, uint64_t kv_heads);
+size_t rbn_kv_open_bytes(uint64_t rows, uint64_t kv_heads, uint64_t head_dim);
+/* Plans one call for all rows from d_new [rows]: n > 0 gives row r n more positions, n = 0 leaves it
+ * alone, n < 0 ends it (its length becomes 0 and its pages go behind the free ones, to be taken
+ * from the next plan on).  Rows are admitted in their order; a row that needs pages gets its tokens only if
+ * the pages needed by it and by the rows before it are free, and only if the tokens so far fit
+ * max_tokens and its own length fits max_blocks; otherwise it is left as it was and RBN_FLAG_KV_REFUSED
+ * is raised (d_start[r+1] - d_start[r] tells how many tokens a row got).  Writes the batch (entries
+ * behind the last token and unit are left alone), the new entries of d_table, the returned pages in
+ * d_ring, and the new lengths and ring state to d_len_out [rows] and d_ring_state_out [2], which may
+ * be table->d_len and table->d_ring_state themselves; if they are not, the call can be repeated
+ * with the same result. */
+int rbn_kv_plan(rbn_ctx *ctx, const rbn_kv_table *table, const int32_t *d_new,
+                const rbn_kv_batch *batch, int32_t *d_len_out, int32_t *d_ring_state_out);
+/* Rotary embedding and K/V store of a planned batch.  d_qkv [max_tokens, (heads + 2 kv_heads) *
+ * head_dim] f32 = (q | k | v), not modified.  Rotates the pairs (i, i + head_dim/2) of q and k by the
+ * angle pos * theta^(-2i/head_dim), evaluated in 64 bits; rotated q goes to d_q [max_tokens, heads *
+ * head_dim] f32 (16-byte aligned), k and v into the cache.  Rows of d_q behind the last token are left alone.
+ * heads is a multiple of kv_heads, at most 1024. */
+int rbn_rope_kv_store_q8(rbn_ctx *ctx, const float *d_qkv, const rbn_kv_table *table,
+                         const rbn_kv_batch *batch, const rbn_kv_layer *layer, uint64_t heads,
+                         float theta, float *d_q);
+/* What the cache holds at `count` places (d_row[i], d_pos[i]), by table->d_len: d_k and d_v
+ * [count, kv_heads, head_dim] f16, the code times the scale rounded once.  A place outside its
+ * row gives zeros and RBN_FLAG_KV_BAD_INDEX. */
+int rbn_kv_read_f16(rbn_ctx *ctx, const rbn_kv_table *table, const rbn_kv_layer *layer,
+                    const int32_t *d_row, const int32_t *d_pos, uint64_t count, void *d_k, void *d_v);
+/* Causal attention of a planned and stored batch over the cache: token i of row r attends to positions
+ * 0 .. d_pos[i] of r, softmax(q.k / sqrt(head_dim)).v; query head h uses K/V head h / (heads /
+ * kv_heads).  d_q is rbn_rope_kv_store_q8's; d_out [max_tokens, heads * head_dim] f32, rows behind the
+ * last token left alone; both 16-byte aligned.  max_new is the most tokens that any row has in the call,
+ * as far as the host knows (1 for a decode step): it picks the kernels, not the result.  A block
+ * whose page is out of range is left out; a token left without any block gets zeros. */
+int rbn_attention_q8kv(rbn_ctx *ctx, const float *d_q, const rbn_kv_table *table,
+                       const rbn_kv_batch *batch, const rbn_kv_layer *layer, uint64_t heads,
+                       uint64_t max_new, float *d_out);
 /* *d_value += delta (the position counter of a captured decode step). */
 int rbn_add_i32(rbn_ctx *ctx, int32_t *d_value, int32_t delta);
 /* Normal(0, sigma) values generated on the device (counter-based, f32 Box-Muller);

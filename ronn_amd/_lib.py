@@ -24,6 +24,15 @@ SUM_TREE = 1
 GEMV_MAX_M = 16
 GEMV_GROUP_MAX = 32
 FLAG_HISTORY_OVERFLOW = 1
+FLAG_KV_REFUSED = 2
+FLAG_KV_BAD_INDEX = 4
+FLAG_KV_NONFINITE = 8
+TOP_MAX = 32
+KV_BLOCK = 32
+KV_MAX_ROWS = 2048
+KV_MAX_BLOCKS = 1 << 20
+KV_MAX_TOKENS = 1 << 18
+KV_I8, KV_E4M3 = 0, 1
 
 # dtype codes of rbn_tensor_bytes (declaration order of the reference's DataType)
 DT_F32, DT_F16, DT_BF16, DT_I8, DT_I32, DT_I64, DT_U8, DT_U32, DT_BOOL, DT_F64 = range(10)
@@ -56,6 +65,48 @@ class GemvProblem(C.Structure):
     ]
 
 
+class KvTable(C.Structure):
+    """rbn_kv_table: page table, lengths and free pages of the rows of a batch (device pointers)."""
+    _fields_ = [
+        ("rows", C.c_uint64),
+        ("max_blocks", C.c_uint64),
+        ("pages", C.c_uint64),
+        ("d_table", C.c_void_p),
+        ("d_len", C.c_void_p),
+        ("d_ring", C.c_void_p),
+        ("d_ring_state", C.c_void_p),
+    ]
+
+
+class KvBatch(C.Structure):
+    """rbn_kv_batch: the tokens of one planned call (device pointers)."""
+    _fields_ = [
+        ("max_tokens", C.c_uint64),
+        ("d_start", C.c_void_p),
+        ("d_row", C.c_void_p),
+        ("d_pos", C.c_void_p),
+        ("d_slot", C.c_void_p),
+        ("d_unit", C.c_void_p),
+        ("d_count", C.c_void_p),
+    ]
+
+
+class KvLayer(C.Structure):
+    """rbn_kv_layer: one layer's 8-bit K/V cache (device pointers)."""
+    _fields_ = [
+        ("format", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("d_k", C.c_void_p),
+        ("d_v", C.c_void_p),
+        ("d_k_open", C.c_void_p),
+        ("d_v_open", C.c_void_p),
+        ("d_k_scale", C.c_void_p),
+        ("d_v_scale", C.c_void_p),
+    ]
+
+
 class RbnError(RuntimeError):
     def __init__(self, code, message):
         super().__init__("%s (rbn status %d)" % (message, code))
@@ -67,6 +118,9 @@ _vp = C.c_void_p
 _u64 = C.c_uint64
 _f32p = C.POINTER(C.c_float)
 _u64p = C.POINTER(C.c_uint64)
+_tab = C.POINTER(KvTable)
+_bat = C.POINTER(KvBatch)
+_lay = C.POINTER(KvLayer)
 
 # name -> (restype, argtypes).  Every symbol include/ronn_bitnet_hip.h declares.
 SIGNATURES = {
@@ -74,6 +128,7 @@ SIGNATURES = {
     "rbn_last_error": (C.c_char_p, []),
     "rbn_device_count": (C.c_int, []),
     "rbn_ctx_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
+    "rbn_ctx_create_on_stream": (C.c_int, [C.c_int, _vp, C.POINTER(_vp)]),
     "rbn_ctx_destroy": (C.c_int, [_vp]),
     "rbn_get_device_info": (C.c_int, [_vp, C.POINTER(DeviceInfo)]),
     "rbn_malloc": (C.c_int, [_vp, C.c_size_t, C.POINTER(_vp)]),
@@ -121,6 +176,14 @@ SIGNATURES = {
     "rbn_argmax_f32": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _vp, _u64]),
     "rbn_greedy_next_f32": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp]),
     "rbn_device_flags": (C.c_int, [_vp, C.POINTER(C.c_uint32)]),
+    "rbn_token_logprobs_f32": (C.c_int, [_vp, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp, _vp]),
+    "rbn_kv_code_bytes": (C.c_size_t, [_u64, _u64, _u64]),
+    "rbn_kv_scale_bytes": (C.c_size_t, [_u64, _u64]),
+    "rbn_kv_open_bytes": (C.c_size_t, [_u64, _u64, _u64]),
+    "rbn_kv_plan": (C.c_int, [_vp, _tab, _vp, _bat, _vp, _vp]),
+    "rbn_rope_kv_store_q8": (C.c_int, [_vp, _vp, _tab, _bat, _lay, _u64, C.c_float, _vp]),
+    "rbn_kv_read_f16": (C.c_int, [_vp, _tab, _lay, _vp, _vp, _u64, _vp, _vp]),
+    "rbn_attention_q8kv": (C.c_int, [_vp, _vp, _tab, _bat, _lay, _u64, _u64, _vp]),
     "rbn_add_i32": (C.c_int, [_vp, _vp, C.c_int32]),
     "rbn_synth_normal_device_f32": (C.c_int, [_vp, _u64, C.c_float, _vp, _u64]),
     "rbn_probe_mfma_i8": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_double)]),

@@ -13,6 +13,7 @@
 struct rbn_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool adopted = false;  // the stream is the caller's (rbn_ctx_create_on_stream)
     hipEvent_t ev_start = nullptr;
     hipEvent_t ev_stop = nullptr;
     hipDeviceProp_t props{};

@@ -89,7 +89,8 @@ int rbn_device_count(void) {
     return n;
 }
 
-int rbn_ctx_create(int device, rbn_ctx **out) {
+// `adopt`: the context runs on the caller's stream instead of one of its own.
+static int create_context(int device, bool adopt, hipStream_t stream, rbn_ctx **out) {
     rbn_clear_error();
     RBN_REQUIRE(out != nullptr, "out is NULL");
     *out = nullptr;
@@ -100,9 +101,16 @@ int rbn_ctx_create(int device, rbn_ctx **out) {
                         e == hipSuccess ? "device count is 0" : hipGetErrorString(e));
     RBN_REQUIRE(device >= 0 && device < n, "device %d out of range [0,%d)", device, n);
     RBN_HIP(hipSetDevice(device));
+    if (adopt && stream) {
+        hipDevice_t on = -1;
+        RBN_HIP(hipStreamGetDevice(stream, &on));
+        RBN_REQUIRE((int)on == device, "the stream belongs to device %d, not %d", (int)on, device);
+    }
     rbn_ctx *ctx = new (std::nothrow) rbn_ctx();
     if (!ctx) return rbn_fail(RBN_ERR_OOM, "host allocation failed");
     ctx->device = device;
+    ctx->adopted = adopt;
+    if (adopt) ctx->stream = stream;
     e = hipGetDeviceProperties(&ctx->props, device);
     if (e != hipSuccess) {
         delete ctx;
@@ -116,7 +124,7 @@ int rbn_ctx_create(int device, rbn_ctx **out) {
                         arch.c_str());
     }
     // Default priority on purpose: one plain non-blocking stream per context.
-    if ((e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking)) != hipSuccess ||
+    if ((!adopt && (e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking)) != hipSuccess) ||
         (e = hipEventCreate(&ctx->ev_start)) != hipSuccess ||
         (e = hipEventCreate(&ctx->ev_stop)) != hipSuccess ||
         (e = hipHostMalloc(&ctx->mailbox, 4096, hipHostMallocDefault)) != hipSuccess ||
@@ -138,10 +146,16 @@ int rbn_ctx_create(int device, rbn_ctx **out) {
     return RBN_OK;
 }
 
+int rbn_ctx_create(int device, rbn_ctx **out) { return create_context(device, false, nullptr, out); }
+
+int rbn_ctx_create_on_stream(int device, void *stream, rbn_ctx **out) {
+    return create_context(device, true, static_cast<hipStream_t>(stream), out);
+}
+
 int rbn_ctx_destroy(rbn_ctx *ctx) {
     if (!ctx) return RBN_OK;
     (void)hipSetDevice(ctx->device);
-    if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
+    if (ctx->stream || ctx->adopted) (void)hipStreamSynchronize(ctx->stream);
     rbn_skinny_release(ctx);
     if (ctx->ws) (void)hipFree(ctx->ws);
     if (ctx->ws2) (void)hipFree(ctx->ws2);
@@ -151,7 +165,7 @@ int rbn_ctx_destroy(rbn_ctx *ctx) {
     if (ctx->dev_flags) (void)hipFree(ctx->dev_flags);
     if (ctx->ev_start) (void)hipEventDestroy(ctx->ev_start);
     if (ctx->ev_stop) (void)hipEventDestroy(ctx->ev_stop);
-    if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
+    if (ctx->stream && !ctx->adopted) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
     return RBN_OK;
 }

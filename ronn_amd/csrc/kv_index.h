@@ -1,0 +1,95 @@
+// Indexing of the paged K/V cache: the descriptors as the kernels get them, page layouts, and the reading
+// of a batch with every number checked against the sizes.  Plain C++, so that it also compiles for
+// the host.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/ronn_bitnet_hip.h"
+
+#ifdef __HIPCC__
+#include <hip/hip_fp16.h>
+#define KV_FN __host__ __device__ __forceinline__
+typedef __half KvHalf;
+#else
+#define KV_FN static inline
+typedef uint16_t KvHalf;
+#endif
+
+constexpr int kKvBlock = RBN_KV_BLOCK;
+
+struct KvTableArgs {
+    int rows, max_blocks, pages;
+    int32_t *table;
+    const int32_t *len;
+    int32_t *ring;
+    const int32_t *ring_state;
+};
+struct KvBatchArgs {
+    int max_tokens;
+    int32_t *start, *row, *pos, *slot, *unit, *count;
+};
+struct KvLayerArgs {
+    int kv_heads;
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    KvHalf *k_open, *v_open;
+};
+
+// Byte of code (t, d) inside a page head, as the matrix instructions read them.
+template <int HD>
+KV_FN int kv_k_byte(int t, int d) {
+    return (((t >> 4) * (HD / 64) + (d >> 6)) * 64 + ((d & 31) >> 3) * 16 + (t & 15)) * 16 + ((d >> 5) & 1) * 8 + (d & 7);
+}
+template <int HD>
+KV_FN int kv_v_byte(int t, int d) {
+    return ((d >> 5) * 64 + ((t & 15) >> 2) * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 + (t >> 4) * 4 + (t & 3);
+}
+
+// What a workgroup needs to know of unit u of a batch.
+struct KvUnit {
+    int row, first;  // first: the unit's first token
+    int n;           // tokens of the unit; 0 if there is nothing (sound) to do
+    int pos;         // position of its first token
+    int row_first;   // the row's first token of the call
+    int row_pos;     // ... and its position
+    int row_n;       // tokens of the row in the call
+};
+
+// *bad is set if what the batch says of the unit does not fit the table and the batch's own sizes.
+KV_FN KvUnit kv_resolve_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, bool *bad) {
+    KvUnit r;
+    r.n = 0;
+    const int tokens = b.count[0] < b.max_tokens ? b.count[0] : b.max_tokens;
+    if (u >= (b.count[1] < b.max_tokens ? b.count[1] : b.max_tokens)) return r;
+    *bad = true;
+    const int i = b.unit[u], cap = t.max_blocks * kKvBlock;
+    if (i < 0 || i >= tokens) return r;
+    r.first = i;
+    r.row = b.row[i];
+    r.pos = b.pos[i];
+    if (r.row < 0 || r.row >= t.rows || r.pos < 0 || r.pos >= cap) return r;
+    r.row_first = b.start[r.row];
+    const int end = b.start[r.row + 1];
+    if (r.row_first < 0 || r.row_first > i || end <= i || end > tokens) return r;
+    r.row_n = end - r.row_first;
+    r.row_pos = r.pos - (i - r.row_first);
+    if (r.row_pos < 0 || r.row_pos + r.row_n > cap) return r;
+    const int left = kKvBlock - (r.pos & (kKvBlock - 1));
+    r.n = end - i < left ? end - i : left;
+    *bad = false;
+    return r;
+}
+
+// Page of a row's block (both in range), or -1.
+KV_FN int kv_page(const KvTableArgs &t, int row, int block) {
+    const int page = t.table[(size_t)row * t.max_blocks + block];
+    return page >= 0 && page < t.pages ? page : -1;
+}
+
+// Page of a slot, or -1.
+KV_FN int kv_slot_page(const KvTableArgs &t, int slot) {
+    const int page = slot / kKvBlock;
+    return slot >= 0 && page < t.pages ? page : -1;
+}

@@ -50,12 +50,16 @@ class DeviceBuffer:
 
 
 class Context:
-    """One GPU, one stream (rbn_ctx)."""
+    """One GPU, one stream (rbn_ctx): its own, or with `stream` the caller's (the integer handle of a
+    HIP stream, e.g. torch.cuda.current_stream().cuda_stream; 0 is the default stream)."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int = None):
         self.lib = _lib.load()
         h = C.c_void_p()
-        check(self.lib.rbn_ctx_create(int(device), C.byref(h)))
+        if stream is None:
+            check(self.lib.rbn_ctx_create(int(device), C.byref(h)))
+        else:
+            check(self.lib.rbn_ctx_create_on_stream(int(device), int(stream) or None, C.byref(h)))
         self.handle = h.value
         self.device = int(device)
 
@@ -86,6 +90,12 @@ class Context:
 
     def sync(self):
         check(self.lib.rbn_sync(self.handle))
+
+    def device_flags(self) -> int:
+        """The RBN_FLAG_* bits that kernels raised since the last call (which clears them)."""
+        flags = C.c_uint32()
+        check(self.lib.rbn_device_flags(self.handle, C.byref(flags)))
+        return flags.value
 
     def device_info(self) -> dict:
         info = _lib.DeviceInfo()

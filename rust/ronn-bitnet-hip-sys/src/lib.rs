@@ -68,6 +68,19 @@ pub const RBN_KERNEL_GEMV: c_int = 0;
 pub const RBN_KERNEL_SKINNY: c_int = 1;
 pub const RBN_KERNEL_MFMA: c_int = 2;
 pub const RBN_FLAG_HISTORY_OVERFLOW: u32 = 1;
+pub const RBN_FLAG_KV_REFUSED: u32 = 2;
+pub const RBN_FLAG_KV_BAD_INDEX: u32 = 4;
+pub const RBN_FLAG_KV_NONFINITE: u32 = 8;
+pub const RBN_TOP_MAX: u64 = 32;
+pub const RBN_KV_BLOCK: u64 = 32;
+pub const RBN_KV_MAX_ROWS: u64 = 2048;
+/// Blocks of one row.
+pub const RBN_KV_MAX_BLOCKS: u64 = 1 << 20;
+/// Tokens of one call.
+pub const RBN_KV_MAX_TOKENS: u64 = 1 << 18;
+// rbn_kv_format
+pub const RBN_KV_I8: u32 = 0;
+pub const RBN_KV_E4M3: u32 = 1;
 pub const RBN_STATIC_SCRATCH_TILES: usize = 1024;
 pub const RBN_STATIC_SCRATCH_BYTES: usize = RBN_STATIC_SCRATCH_TILES * 4096 + 128 * 4;
 
@@ -111,6 +124,46 @@ pub struct rbn_gemv_problem {
     pub reserved: u32,
 }
 
+/// Page table, lengths and free pages of the rows of a batch (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rbn_kv_table {
+    pub rows: u64,
+    pub max_blocks: u64,
+    pub pages: u64,
+    pub d_table: *mut i32,
+    pub d_len: *const i32,
+    pub d_ring: *mut i32,
+    pub d_ring_state: *const i32,
+}
+/// Tokens of one planned call (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rbn_kv_batch {
+    pub max_tokens: u64,
+    pub d_start: *mut i32,
+    pub d_row: *mut i32,
+    pub d_pos: *mut i32,
+    pub d_slot: *mut i32,
+    pub d_unit: *mut i32,
+    pub d_count: *mut i32,
+}
+/// One layer's 8-bit K/V cache (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rbn_kv_layer {
+    pub format: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub reserved: u32,
+    pub d_k: *mut c_void,
+    pub d_v: *mut c_void,
+    pub d_k_open: *mut c_void,
+    pub d_v_open: *mut c_void,
+    pub d_k_scale: *mut f32,
+    pub d_v_scale: *mut f32,
+}
+
 /// `BitNetProviderConfig` (bitnet/provider.rs:41-55) plus `activation`,
 /// `strict_reference_sum` and `device`.
 #[repr(C)]
@@ -134,6 +187,7 @@ extern "C" {
     pub fn rbn_last_error() -> *const c_char;
     pub fn rbn_device_count() -> c_int;
     pub fn rbn_ctx_create(device: c_int, out: *mut *mut rbn_ctx) -> c_int;
+    pub fn rbn_ctx_create_on_stream(device: c_int, stream: *mut c_void, out: *mut *mut rbn_ctx) -> c_int;
     pub fn rbn_ctx_destroy(ctx: *mut rbn_ctx) -> c_int;
     pub fn rbn_get_device_info(ctx: *mut rbn_ctx, out: *mut rbn_device_info) -> c_int;
     pub fn rbn_malloc(ctx: *mut rbn_ctx, bytes: usize, d_out: *mut *mut c_void) -> c_int;
@@ -419,6 +473,60 @@ extern "C" {
         d_table: *const f32,
         H: u64,
         d_x: *mut f32,
+    ) -> c_int;
+    pub fn rbn_token_logprobs_f32(
+        ctx: *mut rbn_ctx,
+        d_logits: *const f32,
+        rows: u64,
+        vocab: u64,
+        pitch: u64,
+        d_target: *const i32,
+        top: u64,
+        d_logprob: *mut f32,
+        d_entropy: *mut f32,
+        d_top_token: *mut i32,
+        d_top_logprob: *mut f32,
+    ) -> c_int;
+    pub fn rbn_kv_code_bytes(pages: u64, kv_heads: u64, head_dim: u64) -> usize;
+    pub fn rbn_kv_scale_bytes(pages: u64, kv_heads: u64) -> usize;
+    pub fn rbn_kv_open_bytes(rows: u64, kv_heads: u64, head_dim: u64) -> usize;
+    pub fn rbn_kv_plan(
+        ctx: *mut rbn_ctx,
+        table: *const rbn_kv_table,
+        d_new: *const i32,
+        batch: *const rbn_kv_batch,
+        d_len_out: *mut i32,
+        d_ring_state_out: *mut i32,
+    ) -> c_int;
+    pub fn rbn_rope_kv_store_q8(
+        ctx: *mut rbn_ctx,
+        d_qkv: *const f32,
+        table: *const rbn_kv_table,
+        batch: *const rbn_kv_batch,
+        layer: *const rbn_kv_layer,
+        heads: u64,
+        theta: f32,
+        d_q: *mut f32,
+    ) -> c_int;
+    pub fn rbn_kv_read_f16(
+        ctx: *mut rbn_ctx,
+        table: *const rbn_kv_table,
+        layer: *const rbn_kv_layer,
+        d_row: *const i32,
+        d_pos: *const i32,
+        count: u64,
+        d_k: *mut c_void,
+        d_v: *mut c_void,
+    ) -> c_int;
+    pub fn rbn_attention_q8kv(
+        ctx: *mut rbn_ctx,
+        d_q: *const f32,
+        table: *const rbn_kv_table,
+        batch: *const rbn_kv_batch,
+        layer: *const rbn_kv_layer,
+        heads: u64,
+        max_new: u64,
+        d_out: *mut f32,
     ) -> c_int;
     pub fn rbn_add_i32(ctx: *mut rbn_ctx, d_value: *mut i32, delta: i32) -> c_int;
     pub fn rbn_synth_normal_device_f32(
