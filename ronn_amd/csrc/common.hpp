@@ -36,6 +36,8 @@ struct rbn_ctx {
     // context and never moved, so launches captured in a HIP graph stay valid.
     void *splitk_partials = nullptr;
     unsigned *splitk_tickets = nullptr;
+    // tickets of the attention over the paged cache: RBN_ATTENTION_ITEMS (item, column tile) pairs
+    unsigned *attention_tickets = nullptr;
     // One word of RBN_FLAG_* bits that kernels set when they refuse to do something a host
     // check could not see coming (rbn_device_flags reads and clears it).
     unsigned *dev_flags = nullptr;
@@ -48,6 +50,7 @@ struct rbn_ctx {
 
 constexpr int RBN_SPLITK_TILES = 16384;  // 64 MiB
 constexpr int RBN_SPLITK_GROUPS = 1024;
+constexpr int RBN_ATTENTION_ITEMS = 4096;
 
 // Records `fmt...` as the calling thread's last error and returns `code`.
 int rbn_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));

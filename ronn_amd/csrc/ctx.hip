@@ -131,6 +131,8 @@ static int create_context(int device, bool adopt, hipStream_t stream, rbn_ctx **
         (e = hipMalloc(&ctx->splitk_partials, (size_t)RBN_SPLITK_TILES * 4096)) != hipSuccess ||
         (e = hipMalloc((void **)&ctx->splitk_tickets, RBN_SPLITK_GROUPS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMemset(ctx->splitk_tickets, 0, RBN_SPLITK_GROUPS * sizeof(unsigned))) != hipSuccess ||
+        (e = hipMalloc((void **)&ctx->attention_tickets, RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
+        (e = hipMemset(ctx->attention_tickets, 0, RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMalloc((void **)&ctx->dev_flags, 256)) != hipSuccess ||
         (e = hipMemset(ctx->dev_flags, 0, 256)) != hipSuccess) {
         int rc = rbn_fail(RBN_ERR_HIP, "context set-up failed: %s", hipGetErrorString(e));
@@ -162,6 +164,7 @@ int rbn_ctx_destroy(rbn_ctx *ctx) {
     if (ctx->mailbox) (void)hipHostFree(ctx->mailbox);
     if (ctx->splitk_partials) (void)hipFree(ctx->splitk_partials);
     if (ctx->splitk_tickets) (void)hipFree(ctx->splitk_tickets);
+    if (ctx->attention_tickets) (void)hipFree(ctx->attention_tickets);
     if (ctx->dev_flags) (void)hipFree(ctx->dev_flags);
     if (ctx->ev_start) (void)hipEventDestroy(ctx->ev_start);
     if (ctx->ev_stop) (void)hipEventDestroy(ctx->ev_stop);
