@@ -5,8 +5,22 @@ namespace {
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+template <int BYTES>
+struct CodeVec {
+    typedef v4u type;
+};
+template <>
+struct CodeVec<8> {
+    typedef v2u type;
+};
+
+constexpr float kLog2eBySqrt128 = 0.12751743082459868f, kLog2eBySqrt64 = 0.18033688011112042f;
 
 // Eight codes as f16, exactly: int8 c is the f16 with bits 0x6400 | (c + 128) (that is 1024 + c +
 // 128) minus 1152; e4m3 has a conversion.
@@ -66,6 +80,7 @@ constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
 constexpr int kMinBlocksPerWave = 2;  // before another workgroup shares an item
 constexpr int kTargetGroups = 4096;
+constexpr int kFewColumns = 16;
 
 // floats of one split's partial result: columns x (out, max, sum)
 template <int HD, int NT>
@@ -75,7 +90,7 @@ constexpr int partial_floats() {
 
 template <int FMT, int HD, int NT, bool PER_TOKEN>
 __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_token_kernel(
-    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int splits,
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int splits, int max_columns,
     float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 32;   // k steps of the scores
     constexpr int DT = HD / 16;   // tiles of dimensions of the output
@@ -101,7 +116,7 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
         if (row < 0 || row >= t.rows) pos = -1;
     } else {
         const KvUnit unit = kv_unit(t, b, u, flags);
-        if (unit.n == 0) return;
+        if (unit.n == 0 || unit.row_n * group > max_columns) return;
         first = unit.first;
         n = unit.n;
         row = unit.row;
@@ -146,7 +161,7 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
             const int ex = exponent_of(m);
-            col_scale[ct] = ldexpf(HD == 128 ? 0.12751743082459868f : 0.18033688011112042f, ex);  // log2(e) / sqrt(hd)
+            col_scale[ct] = ldexpf(HD == 128 ? kLog2eBySqrt128 : kLog2eBySqrt64, ex);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
@@ -388,111 +403,349 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
     }
 }
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
+// ---- many query columns: prompts -------------------------------------------------------------------
+// The same products on v_mfma_f32_32x32x16_f16, a wave with 32 queries (one block of positions of one head)
+// against blocks of 32 keys.
+//  * The (block, head) pairs of a row and a K/V head are numbered block by block; the four waves of a
+//    workgroup take four in a row and share the keys and values, which the workgroup converts
+//    once to f16 in LDS, in operand order: every operand read is one conflict-free 16-byte read per lane.
+//  * The next block's codes are in flight while the present one is used; they are converted into the other LDS
+//    buffer between the scores and the softmax: one barrier per block.
+//  * q and P in f16 as hi + lo, two instructions each (a tile has 32 columns of its own here).  V's scale
+//    goes into P; the output is kept in units of a power of two near the scales so far, with P
+//    shifted up by 2^8, so that neither part of P leaves f16's range: scales within
+//    [2^-4, 4) of the unit use it as it is, others move it (the store's scales span 2^-32 .. 2^9).
+//  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
+constexpr int kPromptThreads = 256;
+constexpr int kPromptTargetGroups = 512;
+constexpr int kPromptMinBlocks = 4;  // before another workgroup shares a tile's keys
 
-// One workgroup per (token, query head).  Each wave takes every fourth block with a running maximum
-// and sum: scores with two lanes per key, then P.V with every lane on its own dimensions; the waves
-// meet through LDS.
+// floats of one workgroup's partial result: four waves' registers, maxima and sums, lane by lane
+template <int HD>
+constexpr int prompt_partial_floats() {
+    return 4 * 64 * (HD / 2 + 2);
+}
+
 template <int FMT, int HD>
-__global__ __launch_bounds__(kThreads) void attention_simple_kernel(const float *__restrict__ q, KvTableArgs t,
-                                                                   KvBatchArgs b, KvLayerArgs l, int heads,
-                                                                   float *__restrict__ out, unsigned *flags) {
-    constexpr int PER = HD / 64;  // dimensions a lane owns in P.V
-    __shared__ float s_q[HD];
-    __shared__ float s_p[kWaves][kKvBlock];
-    __shared__ float s_m[kWaves], s_l[kWaves], s_o[kWaves][HD];
-    const int i = blockIdx.x, h = blockIdx.y, kvh = h / (heads / l.kv_heads);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (i >= min(b.count[0], b.max_tokens)) return;
-    const int row = b.row[i], pos = b.pos[i];
-    const bool ok = row >= 0 && row < t.rows && pos >= 0 && pos < t.max_blocks * kKvBlock;
-    int len = 0;
-    if (ok) {
-        const int end = b.start[row + 1];
-        len = end > i && end <= b.max_tokens ? min(pos + (end - i), t.max_blocks * kKvBlock) : 0;
-    }
-    if (len == 0) {
+__global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int splits, int min_columns,
+    float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+    constexpr int KK = HD / 16;   // k steps of the scores
+    constexpr int NT = HD / 32;   // tiles of dimensions of the output
+    constexpr int kTile = kKvBlock * HD;
+    constexpr int PER = kTile / kPromptThreads;  // codes of K (and of V) a thread converts: 16 or 8
+    __shared__ __attribute__((aligned(16))) _Float16 s_k[2][kTile], s_v[2][kTile];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, g = lane >> 5;
+    const int group = heads / l.kv_heads;
+    const int per_unit = (group + 3) / 4;
+    const int split = blockIdx.x % splits, item = blockIdx.x / splits;
+    const int kvh = item % l.kv_heads, z = item / l.kv_heads % per_unit;
+    const int u = min(b.count[1], b.max_tokens) - 1 - item / l.kv_heads / per_unit;  // the long ones first
+    if (u < 0) return;
+    const KvUnit unit = kv_unit(t, b, u, flags);
+    if (unit.n == 0 || unit.row_n * group < min_columns) return;
+    // the workgroups whose first pair is in this unit
+    const int first_block = unit.row_pos / kKvBlock, last_block = (unit.row_pos + unit.row_n - 1) / kKvBlock;
+    const int nth = unit.pos / kKvBlock - first_block;
+    const int pair0 = (((nth * group + 3) >> 2) + z) * 4;
+    if (pair0 >= (nth + 1) * group) return;
+    const int len = min(t.len[unit.row], t.max_blocks * kKvBlock);
+    if (unit.row_pos + unit.row_n > len) {
         if (tid == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
         return;
     }
-    if (tid < HD) s_q[tid] = q[((size_t)i * heads + h) * HD + tid] * (HD == 128 ? 0.08838834764831845f : 0.125f);
-    __syncthreads();
-    float run_max = -INFINITY, run_sum = 0.0f, o[PER];
-    for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-    for (int blk = wave; blk <= pos / kKvBlock; blk += kWaves) {
-        const bool full = (blk + 1) * kKvBlock <= len;
-        size_t ph = 0;
-        if (full) {
-            const int page = kv_page(t, row, blk);
-            if (page < 0) {
-                if (lane == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
-                continue;
+    const int pairs = (last_block - first_block + 1) * group;
+    const int pair = pair0 + wave;
+    const bool idle = pair >= pairs;
+    const int own = idle ? -1 : first_block + pair / group;               // this wave's block of positions
+    const int top = first_block + min(pair0 + 3, pairs - 1) / group;      // the workgroup's last
+    const int head = kvh * group + (idle ? 0 : pair % group);
+    const int query = own * kKvBlock + col;                               // this lane's position
+    const bool real = !idle && query >= unit.row_pos && query < unit.row_pos + unit.row_n;
+    const int token = unit.row_first + min(max(query - unit.row_pos, 0), unit.row_n - 1);
+    const int full = min(len / kKvBlock, top + 1);                        // full blocks among 0 .. top
+
+    // this workgroup's share of the full blocks; the last share also takes the unfinished block
+    const int shares = max(1, min(splits, full / kPromptMinBlocks));
+    if (split >= shares) return;
+    const int each = (full + shares - 1) / shares;
+    const int from = min(split * each, full), to = min(from + each, full);
+
+    v8h qhi[KK], qlo[KK];
+    float col_scale;
+    {
+        const float *src = q + ((size_t)token * heads + head) * HD + 8 * g;
+        float x[KK][8], m = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const float4 a = *reinterpret_cast<const float4 *>(src + 16 * kk);
+            const float4 c = *reinterpret_cast<const float4 *>(src + 16 * kk + 4);
+            x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = a.z, x[kk][3] = a.w;
+            x[kk][4] = c.x, x[kk][5] = c.y, x[kk][6] = c.z, x[kk][7] = c.w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[kk][e]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const int ex = exponent_of(m);
+        col_scale = ldexpf(HD == 128 ? kLog2eBySqrt128 : kLog2eBySqrt64, ex);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = ldexpf(x[kk][e], -ex);
+                const _Float16 hi = (_Float16)v;
+                qhi[kk][e] = hi;
+                qlo[kk][e] = (_Float16)(v - (float)hi);
             }
-            ph = (size_t)page * l.kv_heads + kvh;
+    }
+
+    float run_max = -INFINITY, run_sum = 0.0f;
+    int vexp = -200;  // exponent of the output's unit; none yet
+    v16f o[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nt][r] = 0.0f;
+
+    // scores of the 32 keys in buffer `buf`: register r is key 8 (r/4) + 4 g + r%4
+    auto scores = [&](int buf) {
+        v16f s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const v8h ka = *reinterpret_cast<const v8h *>(&s_k[buf][(kk * 64 + lane) * 8]);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qhi[kk], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qlo[kk], s, 0, 0, 0);
         }
-        const size_t open = ((size_t)row * l.kv_heads + kvh) * kKvBlock * HD;
-        const int key = lane & 31, part = lane >> 5;
-        float s = 0.0f;
-        for (int d = part * (HD / 2); d < (part + 1) * (HD / 2); ++d)
-            s += s_q[d] * (full ? kv_decode<FMT>(l.k[ph * kKvBlock * HD + kv_k_byte<HD>(key, d)])
-                                : __half2float(l.k_open[open + key * HD + d]));
-        s += __shfl_xor(s, 32);
-        if (full) s *= l.k_scale[ph];
-        const bool seen = blk * kKvBlock + key <= pos;
-        s = seen ? s : -INFINITY;
-        float m = s;
-        for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-        const float new_max = fmaxf(run_max, m);
-        const float p = seen ? __expf(s - new_max) : 0.0f;
-        float sum = p;
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-        const float corr = __expf(run_max - new_max);
-        run_sum = run_sum * corr + sum;
-        run_max = new_max;
-        if (part == 0) s_p[wave][key] = p;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        for (int e = 0; e < PER; ++e) {
-            const int d = lane * PER + e;
-            float acc = 0.0f;
-            for (int j = 0; j < kKvBlock; ++j) {
-                if (blk * kKvBlock + j > pos) break;  // what lies behind may be anything
-                acc += s_p[wave][j] * (full ? kv_decode<FMT>(l.v[ph * kKvBlock * HD + kv_v_byte<HD>(j, d)])
-                                            : __half2float(l.v_open[open + j * HD + d]));
+        return s;
+    };
+    // softmax and P.V of block kb
+    auto attend = [&](v16f s, int buf, float kscale, float vscale, int kb) {
+        // the unit of the output follows V's scale
+        const int ve = exponent_of(vscale);
+        if (vscale > 0.0f && (ve < vexp - 4 || ve > vexp + 1)) {
+            if (vexp > -200) {
+                const float by = ldexpf(1.0f, vexp - ve);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[nt][r] *= by;
             }
-            if (full) acc *= l.v_scale[ph];
-            o[e] = o[e] * corr + acc;
+            vexp = ve;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
-    if (lane == 0) {
-        s_m[wave] = run_max;
-        s_l[wave] = run_sum;
-    }
-    for (int e = 0; e < PER; ++e) s_o[wave][lane * PER + e] = o[e];
-    __syncthreads();
-    if (tid < HD) {
-        float m = -INFINITY, num = 0.0f, den = 0.0f;
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_m[w]);
-        for (int w = 0; w < kWaves; ++w) {
-            const float c = s_m[w] == -INFINITY ? 0.0f : __expf(s_m[w] - m);
-            num += c * s_o[w][tid];
-            den += c * s_l[w];
+        const float shift = ldexpf(vscale, 8 - vexp);
+        const float f = kscale * col_scale;
+        float m = -INFINITY;
+        if (kb == own) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = 8 * (r >> 2) + 4 * g + (r & 3) <= col ? s[r] * f : -INFINITY;
+                m = fmaxf(m, s[r]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] *= f;
+                m = fmaxf(m, s[r]);
+            }
         }
-        out[((size_t)i * heads + h) * HD + tid] = den > 0.0f || den != den ? num / den : 0.0f;
+        if (__any(m > run_max + 4.0f)) {
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float mx = fmaxf(run_max, m);
+            const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
+            run_max = mx;
+            run_sum *= corr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[nt][r] *= corr;
+        }
+        const float ref = run_max == -INFINITY ? 0.0f : run_max;
+        v8h phi[2], plo[2];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(s[r] - ref), p1 = __builtin_amdgcn_exp2f(s[r + 1] - ref);
+            run_sum += p0 + p1;
+            const float w0 = p0 * shift, w1 = p1 * shift;
+            const v2h hi = __builtin_convertvector((v2f){w0, w1}, v2h);
+            const v2h lo = __builtin_convertvector(((v2f){w0 - (float)hi[0], w1 - (float)hi[1]}), v2h);
+            phi[r >> 3][r & 7] = hi[0];
+            phi[r >> 3][(r & 7) + 1] = hi[1];
+            plo[r >> 3][r & 7] = lo[0];
+            plo[r >> 3][(r & 7) + 1] = lo[1];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const v8h va = *reinterpret_cast<const v8h *>(&s_v[buf][((nt * 2 + s2) * 64 + lane) * 8]);
+                o[nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, phi[s2], o[nt], 0, 0, 0);
+                o[nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, plo[s2], o[nt], 0, 0, 0);
+            }
+    };
+
+    // ---- the unfinished block first, if it is this share's: f16, rows behind the end zeroed
+    if (top >= full && split == shares - 1) {
+        const size_t at = ((size_t)unit.row * l.kv_heads + kvh) * kTile;
+        const _Float16 *ko = reinterpret_cast<const _Float16 *>(l.k_open) + at;
+        const _Float16 *vo = reinterpret_cast<const _Float16 *>(l.v_open) + at;
+        const int valid = len - full * kKvBlock;
+        for (int i = tid; i < kTile / 8; i += kPromptThreads) {
+            const int key = i / (HD / 8), d = i % (HD / 8) * 8;
+            v8h kx = *reinterpret_cast<const v8h *>(ko + key * HD + d), vx = *reinterpret_cast<const v8h *>(vo + key * HD + d);
+            if (key >= valid) kx = vx = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+            *reinterpret_cast<v8h *>(&s_k[0][((d >> 4) * 64 + 32 * ((d >> 3) & 1) + key) * 8]) = kx;
+            const int quad = (key & 15) >> 2, e = 4 * (quad >> 1) + (key & 3);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s_v[0][(((d >> 5) * 2 + (key >> 4)) * 64 + 32 * (quad & 1) + ((d + j) & 31)) * 8 + e] = vx[j];
+        }
+        __syncthreads();
+        if (own == top) attend(scores(0), 0, 1.0f, 1.0f, top);
+        __syncthreads();
     }
+
+    // ---- the share's full blocks
+    typedef typename CodeVec<PER>::type vcode;  // a thread's codes of one page head
+    vcode kc, vc;
+    auto load = [&](int page) {  // (an invalid page loads page 0 and is skipped)
+        const size_t at = ((size_t)max(page, 0) * l.kv_heads + kvh) * kTile + tid * PER;
+        kc = *reinterpret_cast<const vcode *>(l.k + at);
+        vc = *reinterpret_cast<const vcode *>(l.v + at);
+    };
+    auto convert = [&](int buf) {
+        // code byte offset of this thread and what it is: see kv_k_byte and kv_v_byte
+#pragma unroll
+        for (int h = 0; h < PER / 8; ++h) {
+            const int byte = tid * PER + 8 * h;
+            const int chunk = byte >> 4, hh = (byte >> 3) & 1;
+            {
+                const int i = chunk & 15, gg = (chunk >> 4) & 3, aj = chunk >> 6, a = aj / (HD / 64), j = aj % (HD / 64);
+                const int kk = (2 * j + hh) * 2 + (gg >> 1);
+                *reinterpret_cast<v8h *>(&s_k[buf][(kk * 64 + 32 * (gg & 1) + 16 * a + i) * 8]) =
+                    codes_to_f16<FMT>(kc[2 * h], kc[2 * h + 1]);
+            }
+            {
+                const int i = chunk & 15, quad = (chunk >> 4) & 3, p = chunk >> 6;
+                const v8h x = codes_to_f16<FMT>(vc[2 * h], vc[2 * h + 1]);  // keys 4 quad .. +3, then 16 + 4 quad ..
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+                    *reinterpret_cast<v4h *>(&s_v[buf][((p * 2 + a) * 64 + 32 * (quad & 1) + 16 * hh + i) * 8 + 4 * (quad >> 1)]) =
+                        a ? __builtin_shufflevector(x, x, 4, 5, 6, 7) : __builtin_shufflevector(x, x, 0, 1, 2, 3);
+            }
+        }
+    };
+    int page = -1;
+    float ks = 0.0f, vs = 0.0f;
+    auto look_up = [&](int base) {  // pages and scales of blocks base .. base + 63, one per lane
+        page = -1;
+        ks = vs = 0.0f;
+        if (base + lane < to) {
+            page = kv_page(t, unit.row, base + lane);
+            const size_t ph = (size_t)max(page, 0) * l.kv_heads + kvh;
+            ks = l.k_scale[ph];
+            vs = l.v_scale[ph];
+            if (page < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+        }
+    };
+    for (int base = from; base < to; base += 64) {
+        look_up(base);
+        const int steps = min(64, to - base);
+        load(__builtin_amdgcn_readlane(page, 0));
+        convert(0);
+        load(__builtin_amdgcn_readlane(page, min(1, steps - 1)));
+        __syncthreads();
+        for (int i = 0; i < steps; ++i) {
+            const int kb = base + i, buf = i & 1;
+            const bool take = kb <= own && __builtin_amdgcn_readlane(page, i) >= 0;
+            v16f s;
+            if (take) s = scores(buf);
+            if (i + 1 < steps) {
+                convert(buf ^ 1);
+                load(__builtin_amdgcn_readlane(page, min(i + 2, steps - 1)));
+            }
+            if (take)
+                attend(s, buf, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), i)),
+                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), i)), kb);
+            __syncthreads();
+        }
+    }
+
+    run_sum += __shfl_xor(run_sum, 32);
+    const float unit_out = vexp > -200 ? ldexpf(1.0f, vexp - 8) : 0.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nt][r] *= unit_out;
+    if (shares > 1) {
+        float *part = partials + (size_t)item * splits * prompt_partial_floats<HD>();
+        float *mine = part + (size_t)split * prompt_partial_floats<HD>() + wave * 64 * (HD / 2 + 2) + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) store_agent(mine + 64 * (nt * 16 + r), o[nt][r]);
+        store_agent(mine + 64 * (HD / 2), run_max);
+        store_agent(mine + 64 * (HD / 2 + 1), run_sum);
+        // published once the stores have completed (vmcnt(0): this wave's, the barrier: everybody's)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            const int is_last = atomicAdd(&tickets[item], 1u) == (unsigned)shares - 1;
+            if (is_last) atomicExch(&tickets[item], 0u);  // ready for the next launch
+            s_last = is_last;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        const float *from_part = part + wave * 64 * (HD / 2 + 2) + lane;
+        float m = -INFINITY;
+        for (int sp = 0; sp < shares; ++sp)
+            m = fmaxf(m, load_agent(from_part + (size_t)sp * prompt_partial_floats<HD>() + 64 * (HD / 2)));
+        run_sum = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[nt][r] = 0.0f;
+        for (int sp = 0; sp < shares; ++sp) {
+            const float *p = from_part + (size_t)sp * prompt_partial_floats<HD>();
+            const float pm = load_agent(p + 64 * (HD / 2)), pl = load_agent(p + 64 * (HD / 2 + 1));
+            // a share without keys for this query has sum 0; one with nothing but NaN maximum -inf and a NaN sum
+            const float k = pm == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pm - m);
+            run_sum += k * pl;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[nt][r] += k * load_agent(p + 64 * (nt * 16 + r));
+        }
+    }
+    if (!real) return;
+    const float inv = run_sum > 0.0f || run_sum != run_sum ? 1.0f / run_sum : 0.0f;
+    float *dst = out + ((size_t)token * heads + head) * HD + 4 * g;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+            *reinterpret_cast<float4 *>(dst + 32 * nt + 8 * r4) =
+                make_float4(o[nt][4 * r4] * inv, o[nt][4 * r4 + 1] * inv, o[nt][4 * r4 + 2] * inv, o[nt][4 * r4 + 3] * inv);
 }
 
+// What a launch needs besides the descriptors: the columns (tokens x heads of a K/V head) an item is expected
+// to have at most, and the most a row may have to be taken by the first kernel (all others by the second).
+struct AttentionShape {
+    uint32_t head_dim, format;
+    int heads;
+    bool per_token;
+    uint64_t columns;
+    int max_columns;
+};
 
 template <int FMT, int HD, int NT, bool PER_TOKEN>
 int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                    int heads, uint64_t max_new, float *d_out) {
-    const uint64_t group = heads / l.kv_heads;
+                    const AttentionShape &shape, float *d_out) {
     const uint64_t items = (uint64_t)(PER_TOKEN ? (unsigned)b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
-    const uint64_t columns = group * (PER_TOKEN ? 1 : max_new < kKvBlock ? max_new : kKvBlock);
-    const uint64_t tiles = (columns + 8 * NT - 1) / (8 * NT);
+    const uint64_t tiles = (shape.columns + 8 * NT - 1) / (8 * NT);
     // Workgroups that share an item: enough to fill the chip several times over (rows differ in length, and
     // short ones leave their share early), as far as tickets and partial results have room.
     uint64_t splits = kTargetGroups / (items * tiles);
@@ -504,28 +757,52 @@ int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const 
     RBN_REQUIRE(items * splits < (1ull << 31), "too many tokens in rbn_attention_q8kv");
     attention_token_kernel<FMT, HD, NT, PER_TOKEN>
         <<<dim3((unsigned)(items * splits), (unsigned)tiles), dim3(kTokenThreads), 0, ctx->stream>>>(
-            d_q, t, b, l, heads, (int)splits, (float *)ctx->splitk_partials, ctx->attention_tickets, d_out, ctx->dev_flags);
+            d_q, t, b, l, shape.heads, (int)splits, shape.max_columns, (float *)ctx->splitk_partials,
+            ctx->attention_tickets, d_out, ctx->dev_flags);
     RBN_HIP(hipGetLastError());
     return RBN_OK;
 }
 
 template <int FMT, int HD>
 int launch_token_of(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                    int heads, uint64_t max_new, float *d_out) {
-    const uint64_t group = heads / l.kv_heads;
-    if (max_new == 1)
-        return group <= 8 ? launch_token_as<FMT, HD, 1, true>(ctx, d_q, t, b, l, heads, max_new, d_out)
-                          : launch_token_as<FMT, HD, 2, true>(ctx, d_q, t, b, l, heads, max_new, d_out);
-    return group * max_new <= 8 ? launch_token_as<FMT, HD, 1, false>(ctx, d_q, t, b, l, heads, max_new, d_out)
-                                : launch_token_as<FMT, HD, 2, false>(ctx, d_q, t, b, l, heads, max_new, d_out);
+                    const AttentionShape &shape, float *d_out) {
+    auto f = shape.per_token ? (shape.columns <= 8 ? launch_token_as<FMT, HD, 1, true> : launch_token_as<FMT, HD, 2, true>)
+                             : (shape.columns <= 8 ? launch_token_as<FMT, HD, 1, false> : launch_token_as<FMT, HD, 2, false>);
+    return f(ctx, d_q, t, b, l, shape, d_out);
 }
 
 int launch_token(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                 const rbn_kv_layer &layer, int heads, uint64_t max_new, float *d_out) {
-    auto f = layer.format == RBN_KV_I8
-                 ? (layer.head_dim == 128 ? launch_token_of<RBN_KV_I8, 128> : launch_token_of<RBN_KV_I8, 64>)
-                 : (layer.head_dim == 128 ? launch_token_of<RBN_KV_E4M3, 128> : launch_token_of<RBN_KV_E4M3, 64>);
-    return f(ctx, d_q, t, b, l, heads, max_new, d_out);
+                 const AttentionShape &shape, float *d_out) {
+    auto f = shape.format == RBN_KV_I8
+                 ? (shape.head_dim == 128 ? launch_token_of<RBN_KV_I8, 128> : launch_token_of<RBN_KV_I8, 64>)
+                 : (shape.head_dim == 128 ? launch_token_of<RBN_KV_E4M3, 128> : launch_token_of<RBN_KV_E4M3, 64>);
+    return f(ctx, d_q, t, b, l, shape, d_out);
+}
+
+template <int FMT, int HD>
+int launch_prompt_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
+                     const AttentionShape &shape, float *d_out) {
+    const uint64_t group = shape.heads / l.kv_heads;
+    const uint64_t items = (uint64_t)kv_max_units(b.max_tokens, t.rows) * l.kv_heads * ((group + 3) / 4);
+    // Too few tiles to fill the chip: several workgroups share a tile's keys.
+    uint64_t splits = kPromptTargetGroups / items;
+    const uint64_t room = (uint64_t)RBN_SPLITK_TILES * 1024 / (items * prompt_partial_floats<HD>());
+    splits = splits < room ? splits : room;
+    if (splits < 1 || items > RBN_ATTENTION_ITEMS) splits = 1;
+    RBN_REQUIRE(items * splits < (1ull << 31), "too many tokens in rbn_attention_q8kv");
+    attention_prompt_kernel<FMT, HD><<<dim3((unsigned)(items * splits)), dim3(kPromptThreads), 0, ctx->stream>>>(
+        d_q, t, b, l, shape.heads, (int)splits, shape.max_columns + 1, (float *)ctx->splitk_partials, ctx->attention_tickets, d_out,
+        ctx->dev_flags);
+    RBN_HIP(hipGetLastError());
+    return RBN_OK;
+}
+
+int launch_prompt(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
+                  const AttentionShape &shape, float *d_out) {
+    auto f = shape.format == RBN_KV_I8
+                 ? (shape.head_dim == 128 ? launch_prompt_as<RBN_KV_I8, 128> : launch_prompt_as<RBN_KV_I8, 64>)
+                 : (shape.head_dim == 128 ? launch_prompt_as<RBN_KV_E4M3, 128> : launch_prompt_as<RBN_KV_E4M3, 64>);
+    return f(ctx, d_q, t, b, l, shape, d_out);
 }
 
 }  // namespace
@@ -548,17 +825,14 @@ int rbn_attention_q8kv(rbn_ctx *ctx, const float *d_q, const rbn_kv_table *table
                 layer->kv_heads);
     RBN_REQUIRE(max_new > 0, "max_new of rbn_attention_q8kv is 0");
     RBN_ENTER(ctx);
+    // Rows with few columns go to the first kernel, the others to the second; where the host knows that there
+    // are only few, the second is not launched and the first takes all.
     const uint64_t group = heads / layer->kv_heads;
-    if (max_new * group <= 16) {
-        return launch_token(ctx, d_q, t, b, l, *layer, (int)heads, max_new, d_out);
-    }
-    auto kernel =
-        layer->format == RBN_KV_I8
-            ? (layer->head_dim == 128 ? attention_simple_kernel<RBN_KV_I8, 128> : attention_simple_kernel<RBN_KV_I8, 64>)
-            : (layer->head_dim == 128 ? attention_simple_kernel<RBN_KV_E4M3, 128> : attention_simple_kernel<RBN_KV_E4M3, 64>);
-    kernel<<<dim3((unsigned)batch->max_tokens, (unsigned)heads), dim3(kThreads), 0, ctx->stream>>>(
-        d_q, t, b, l, (int)heads, d_out, ctx->dev_flags);
-    RBN_HIP(hipGetLastError());
+    const bool few = max_new == 1 || max_new * group <= kFewColumns;
+    AttentionShape shape{layer->head_dim, layer->format, (int)heads, max_new == 1, few ? max_new * group : kFewColumns,
+                         few ? INT32_MAX : kFewColumns};
+    RBN_CHECK(launch_token(ctx, d_q, t, b, l, shape, d_out));
+    if (!few) RBN_CHECK(launch_prompt(ctx, d_q, t, b, l, shape, d_out));
     return RBN_OK;
 }
 
