@@ -8,6 +8,9 @@ LLaMA / BitNet-b1.58 ones; tests/decoder_model.py restates them in numpy.
 
 A decode step is 122 kernel launches; it reads the position and the previous token from
 device memory, so it is captured once in a HIP graph and replayed per token.
+
+BitNetDecoder serves one sequence over contiguous f16 caches; BatchDecoder serves several at once
+with the same weights over the paged 8-bit cache (kvcache.py), with log probabilities.
 """
 from __future__ import annotations
 
@@ -20,6 +23,7 @@ import numpy as np
 from . import _lib
 from ._lib import check
 from .device import Context, DeviceBuffer
+from .kvcache import PagedKVCache
 
 
 @dataclasses.dataclass
@@ -33,14 +37,24 @@ class DecoderConfig:
     max_seq: int = 1024
     eps: float = 1e-5
     rope_theta: float = 10000.0
+    kv_heads: int = 0       # K/V heads; 0: as many as query heads.  Fewer are served by BatchDecoder only
+
+    def __post_init__(self):
+        self.kv_heads = self.kv_heads or self.heads
+        if self.kv_heads < 0 or self.heads % self.kv_heads:
+            raise ValueError("heads (%d) must be a multiple of kv_heads (%d)" % (self.heads, self.kv_heads))
 
     @property
     def attn_dim(self) -> int:
         return self.heads * self.head_dim
 
+    @property
+    def qkv_dim(self) -> int:
+        return (self.heads + 2 * self.kv_heads) * self.head_dim
+
     def linear_shapes(self):
         """(name, K, N) of the four BitLinear layers of a block."""
-        return (("wqkv", self.hidden, 3 * self.attn_dim), ("wo", self.attn_dim, self.hidden),
+        return (("wqkv", self.hidden, self.qkv_dim), ("wo", self.attn_dim, self.hidden),
                 ("wgu", self.hidden, 2 * self.ffn), ("wdown", self.ffn, self.hidden))
 
     def packed_weight_bytes_per_token(self) -> int:
@@ -66,7 +80,7 @@ class BitNetDecoder:
         self.x = a(4 * T * H)
         self.o = a(4 * T * H)
         self.d = a(4 * T * H)
-        self.qkv = a(4 * T * 3 * A)
+        self.qkv = a(4 * T * cfg.qkv_dim)
         self.att = a(4 * T * A)
         self.gu = a(4 * T * 2 * F)
         self.logits = a(4 * V)
@@ -75,9 +89,11 @@ class BitNetDecoder:
         self.tokens = a(4 * T)
         self.pos = a(4)
         self.history = a(4 * cfg.max_seq)
+        # the f16 caches; grouped K/V heads have none (BatchDecoder brings its own)
         cache = 2 * cfg.heads * cfg.max_seq * cfg.head_dim
-        self.kcache = [a(cache) for _ in range(cfg.layers)]
-        self.vcache = [a(cache) for _ in range(cfg.layers)]
+        layers = cfg.layers if cfg.kv_heads == cfg.heads else 0
+        self.kcache = [a(cache) for _ in range(layers)]
+        self.vcache = [a(cache) for _ in range(layers)]
         self.blocks = []
         self.embed = self.g_final = self.lm_head = None
         self._graph = None
@@ -96,7 +112,7 @@ class BitNetDecoder:
 
     def load_weights(self, w: dict):
         """w: numpy arrays 'embed' [V,H], 'g_final' [H], 'lm_head' [H,V], and per layer i
-        'L{i}.g_attn' [H], 'L{i}.wqkv' [H,3A], 'L{i}.g_attn_sub' [A], 'L{i}.wo' [A,H],
+        'L{i}.g_attn' [H], 'L{i}.wqkv' [H, qkv_dim], 'L{i}.g_attn_sub' [A], 'L{i}.wo' [A,H],
         'L{i}.g_ffn' [H], 'L{i}.wgu' [H,2F], 'L{i}.g_ffn_sub' [F], 'L{i}.wdown' [F,H]."""
         cfg = self.cfg
 
@@ -242,6 +258,9 @@ class BitNetDecoder:
     def prefill(self, prompt: np.ndarray):
         """Runs the prompt from position 0.  The token predicted after it goes to history slot
         len(prompt), so the prompt has to be shorter than max_seq."""
+        if self.cfg.kv_heads != self.cfg.heads:
+            raise ValueError("a decoder with %d K/V heads for %d query heads is served by BatchDecoder"
+                             % (self.cfg.kv_heads, self.cfg.heads))
         prompt = np.ascontiguousarray(prompt, dtype=np.int32)
         if prompt.ndim != 1 or len(prompt) == 0:
             raise ValueError("the prompt must be a non-empty vector of token ids")
@@ -290,3 +309,249 @@ class BitNetDecoder:
 
     def last_logits(self) -> np.ndarray:
         return self.logits.download(np.float32, self.cfg.vocab)
+
+
+@dataclasses.dataclass
+class NextToken:
+    """What the model says of the token after a row's last one: the greedy choice, its log probability, the
+    entropy (nats) of the distribution, and the `top` most probable tokens with their log probabilities."""
+    token: int
+    logprob: float
+    entropy: float
+    top_tokens: np.ndarray
+    top_logprobs: np.ndarray
+
+
+class BatchDecoder:
+    """Several sequences at once with the weights of a BitNetDecoder, over a paged 8-bit K/V cache.
+
+    A row is the place of one sequence (0 .. rows - 1): start() puts prompts into free rows, step() advances every
+    running row by its greedy token, finish() frees rows.  score() gives the log probabilities of given tokens.
+    pages: pages of 32 positions shared by the rows (0: enough for every row at cfg.max_seq); max_tokens: the most
+    tokens of one call; top: alternatives that come with every token (1 to 32)."""
+
+    LOGIT_ROWS = 256    # rows of logits computed at a time when prompts are scored
+
+    def __init__(self, dec: BitNetDecoder, rows: int, pages: int = 0, max_tokens: int = 512, fmt: str = "i8", top: int = 1):
+        cfg, ctx = dec.cfg, dec.ctx
+        if not dec.blocks:
+            raise ValueError("the decoder has no weights yet")
+        if not 1 <= top <= _lib.TOP_MAX:
+            raise ValueError("top must be in [1, %d]" % _lib.TOP_MAX)
+        if rows < 1 or max_tokens < rows:
+            raise ValueError("max_tokens (%d) must hold one token of each of the %d rows" % (max_tokens, rows))
+        self.dec, self.cfg, self.ctx, self.lib = dec, cfg, ctx, ctx.lib
+        self.rows, self.max_tokens, self.top = rows, max_tokens, top
+        pages = pages or rows * -(-cfg.max_seq // _lib.KV_BLOCK)
+        self.cache = PagedKVCache(ctx, cfg.layers, cfg.kv_heads, cfg.head_dim, rows, pages, cfg.max_seq, max_tokens, fmt)
+        H, A, F, V, T = cfg.hidden, cfg.attn_dim, cfg.ffn, cfg.vocab, max_tokens
+        a = ctx.alloc
+        self.x, self.o, self.d = a(4 * T * H), a(4 * T * H), a(4 * T * H)
+        self.qkv, self.q, self.att, self.gu = a(4 * T * cfg.qkv_dim), a(4 * T * A), a(4 * T * A), a(4 * T * 2 * F)
+        self.pitch = ctx.act_pitch(max(H, A, F))
+        self.acts = (a(T * self.pitch), a(4 * T), a(4 * T))
+        self.last = (a(rows * self.pitch), a(4 * rows), a(4 * rows))   # the last token of each row, for the logits
+        self.tokens, self.targets = a(4 * T), a(4 * max(T, rows))
+        self.d_new = a(4 * rows)
+        self.logit_rows = max(rows, min(T, self.LOGIT_ROWS))
+        R = self.logit_rows
+        self.logits = a(4 * R * V)
+        # one buffer for what comes back: log probability, entropy, top tokens, top log probabilities
+        self.stats = a(4 * R * (2 + 2 * top))
+        self._graphs = {}
+        self._len = np.zeros(rows, dtype=np.int64)     # host copies of what the device holds
+        self._free = pages
+        self._next = {}                                # running rows: their NextToken
+
+    # -- queueing ------------------------------------------------------------------------------------
+    def _forward(self, M: int, max_new: int):
+        """self.tokens[0:M], planned by self.d_new, through all layers; leaves the quantised, normalised last hidden
+        state of every token in self.acts."""
+        cfg, dec, cache = self.cfg, self.dec, self.cache
+        H, A, F = cfg.hidden, cfg.attn_dim, cfg.ffn
+        batch = cache.batch(M)
+        cache.plan(self.d_new, batch)
+        check(self.lib.rbn_embed_f32(self.ctx.handle, dec.embed.ptr, self.tokens.ptr, M, H, cfg.vocab, self.x.ptr))
+        pending = None
+        for i, b in enumerate(dec.blocks):
+            self._norm_quant(self.x, pending, b["g_attn"], M, H)
+            self._linear(b["wqkv"], M, self.qkv)
+            cache.store(i, self.qkv, cfg.heads, cfg.rope_theta, self.q, batch)
+            cache.attend(i, self.q, cfg.heads, max_new, self.att, batch)
+            self._norm_quant(self.att, None, b["g_attn_sub"], M, A)
+            self._linear(b["wo"], M, self.o)
+            self._norm_quant(self.x, self.o, b["g_ffn"], M, H)
+            self._linear(b["wgu"], M, self.gu)
+            self._norm_quant(None, None, b["g_ffn_sub"], M, F, gate_up=self.gu)
+            self._linear(b["wdown"], M, self.d)
+            pending = self.d
+        self._norm_quant(self.x, pending, dec.g_final, M, H)
+
+    def _norm_quant(self, x, delta, gamma, M, H, gate_up=None):
+        check(self.lib.rbn_rmsnorm_quant_i8(
+            self.ctx.handle, x.ptr if x is not None else None, delta.ptr if delta is not None else None,
+            gate_up.ptr if gate_up is not None else None, gamma.ptr, self.cfg.eps, M, H, self.acts[0].ptr,
+            self.acts[1].ptr, self.acts[2].ptr))
+
+    def _linear(self, lin, M, out):
+        self.ctx.matmul(self.acts, lin.tiled, lin.scale, M, lin.K, lin.N, d_out=out)
+
+    def _logprobs(self, acts, row0: int, M: int, with_targets: bool):
+        """Logits of rows row0 .. row0 + M of acts, and what self.stats holds of them."""
+        head, V, top, R = self.dec.lm_head, self.cfg.vocab, self.top, self.logit_rows
+        q, s, r = acts
+        check(self.lib.rbn_matmul_t2_i8(self.ctx.handle, q.ptr + row0 * self.ctx.act_pitch(head.K), s.ptr + 4 * row0,
+                                        r.ptr + 4 * row0, head.tiled.ptr, head.scale, M, head.K, V, None, self.logits.ptr))
+        lp = self.stats.ptr
+        check(self.lib.rbn_token_logprobs_f32(
+            self.ctx.handle, self.logits.ptr, M, V, V, self.targets.ptr + 4 * row0 if with_targets else None, top,
+            lp if with_targets else None, lp + 4 * R, lp + 8 * R, lp + 4 * R * (2 + top)))
+
+    def _fetch(self, M: int):
+        """(log probabilities of the targets, entropies, top tokens [M, top], their log probabilities)."""
+        top, R = self.top, self.logit_rows
+        raw = self.stats.download(np.uint32, R * (2 + 2 * top))
+        tok = raw[2 * R:2 * R + M * top].view(np.int32).reshape(M, top)
+        lps = raw[R * (2 + top):R * (2 + top) + M * top].view(np.float32).reshape(M, top)
+        return raw[:M].view(np.float32).copy(), raw[R:R + M].view(np.float32).copy(), tok.copy(), lps.copy()
+
+    # -- what the host knows before it queues anything --------------------------------------------------
+    def _admit(self, new: dict):
+        """Checks and books `new` tokens per row, so that no row is refused on the device."""
+        total = sum(new.values())
+        if total > self.max_tokens:
+            raise ValueError("%d tokens in one call: max_tokens is %d" % (total, self.max_tokens))
+        blocks = lambda n: -(-int(n) // _lib.KV_BLOCK)  # noqa: E731
+        need = 0
+        for r, n in new.items():
+            if self._len[r] + n > self.cfg.max_seq:
+                raise ValueError("row %d would hold %d positions: max_seq is %d" % (r, self._len[r] + n, self.cfg.max_seq))
+            need += blocks(self._len[r] + n) - blocks(self._len[r])
+        if need > self._free:
+            raise ValueError("%d pages are needed, %d are free" % (need, self._free))
+        self._free -= need
+        for r, n in new.items():
+            self._len[r] += n
+        counts = np.zeros(self.rows, dtype=np.int32)
+        for r, n in new.items():
+            counts[r] = n
+        self.d_new.upload(counts)
+        return total
+
+    def _release(self, rows):
+        counts = np.zeros(self.rows, dtype=np.int32)
+        for r in rows:
+            counts[r] = -1
+            self._free += -(-int(self._len[r]) // _lib.KV_BLOCK)
+            self._len[r] = 0
+        self.d_new.upload(counts)
+        self.cache.plan(self.d_new)
+
+    def _prompts(self, prompts: dict) -> dict:
+        out = {}
+        for r, ids in sorted(prompts.items()):
+            ids = np.ascontiguousarray(ids, dtype=np.int32)
+            if not 0 <= r < self.rows:
+                raise ValueError("row %d is outside [0, %d)" % (r, self.rows))
+            if r in self._next:
+                raise ValueError("row %d is running" % r)
+            if ids.ndim != 1 or ids.size == 0:
+                raise ValueError("a prompt must be a non-empty vector of token ids")
+            out[r] = ids
+        if not out:
+            raise ValueError("no prompts")
+        return out
+
+    # -- serving -------------------------------------------------------------------------------------
+    @property
+    def running(self) -> dict:
+        """Running rows and the token each of them will take next."""
+        return dict(self._next)
+
+    def start(self, prompts: dict) -> dict:
+        """Puts prompts (row -> token ids) into free rows; returns row -> NextToken."""
+        prompts = self._prompts(prompts)
+        self._admit({r: ids.size for r, ids in prompts.items()})
+        ids = np.concatenate(list(prompts.values()))
+        self.tokens.upload(ids)
+        self._forward(ids.size, max(p.size for p in prompts.values()))
+        # the last token of each prompt
+        pitch = self.ctx.act_pitch(self.cfg.hidden)
+        ends = np.cumsum([p.size for p in prompts.values()]) - 1
+        for i, e in enumerate(ends):
+            for src, dst, n in zip(self.acts, self.last, (pitch, 4, 4)):
+                check(self.lib.rbn_d2d(self.ctx.handle, dst.ptr + i * n, src.ptr + int(e) * n, n))
+        self._logprobs(self.last, 0, len(ends), False)
+        return self._took(list(prompts), *self._fetch(len(ends))[1:])
+
+    def _took(self, rows, entropy, tok, lps) -> dict:
+        got = {r: NextToken(int(tok[i, 0]), float(lps[i, 0]), float(entropy[i]), tok[i], lps[i]) for i, r in enumerate(rows)}
+        self._next.update(got)
+        return got
+
+    def step(self, use_graph: bool = True) -> dict:
+        """Appends its next token to every running row; returns row -> NextToken (the one after it).  The step of a
+        number of running rows is captured once and replayed."""
+        rows = sorted(self._next)
+        if not rows:
+            raise ValueError("no row is running")
+        M = self._admit({r: 1 for r in rows})
+        self.tokens.upload(np.array([self._next[r].token for r in rows], dtype=np.int32))
+        if use_graph and M not in self._graphs:
+            self.ctx.graph_begin()
+            try:
+                self._queue_step(M)
+            finally:
+                g = self.ctx.graph_end()
+            self._graphs[M] = g
+        if use_graph:
+            self.ctx.graph_launch(self._graphs[M])
+        else:
+            self._queue_step(M)
+        return self._took(rows, *self._fetch(M)[1:])
+
+    def _queue_step(self, M: int):
+        self._forward(M, 1)
+        self._logprobs(self.acts, 0, M, False)
+
+    def finish(self, rows):
+        """Ends rows; their pages are free again."""
+        rows = [rows] if isinstance(rows, (int, np.integer)) else list(rows)
+        if len(set(rows)) != len(rows) or any(r not in self._next for r in rows):
+            raise ValueError("rows %s are not all running" % rows)
+        self._release(rows)
+        for r in rows:
+            del self._next[r]
+
+    def score(self, prompts: dict):
+        """Log probabilities of given tokens: for each prompt (row -> token ids, free rows) the log probability of its
+        tokens 1 .. and the entropy before each of them: row -> (logprobs [n-1], entropies [n-1]).  The rows are
+        free again afterwards."""
+        prompts = self._prompts(prompts)
+        self._admit({r: ids.size for r, ids in prompts.items()})
+        ids = np.concatenate(list(prompts.values()))
+        # token i is followed by token i + 1 of its own prompt; the last one has no target
+        targets = np.concatenate([np.append(p[1:], -1) for p in prompts.values()]).astype(np.int32)
+        self.tokens.upload(ids)
+        self.targets.upload(targets)
+        self._forward(ids.size, max(p.size for p in prompts.values()))
+        lp, ent = [], []
+        for at in range(0, ids.size, self.logit_rows):
+            n = min(self.logit_rows, ids.size - at)
+            self._logprobs(self.acts, at, n, True)
+            got = self._fetch(n)
+            lp.append(got[0])
+            ent.append(got[1])
+        self._release(list(prompts))
+        lp, ent = np.concatenate(lp), np.concatenate(ent)
+        out, at = {}, 0
+        for r, p in prompts.items():
+            out[r] = (lp[at:at + p.size - 1], ent[at:at + p.size - 1])
+            at += p.size
+        return out
+
+    def close(self):
+        """Destroys the captured steps."""
+        for g in self._graphs.values():
+            self.ctx.graph_destroy(g)
+        self._graphs = {}
