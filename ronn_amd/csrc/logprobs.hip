@@ -3,8 +3,17 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
+constexpr int kVecs = 8;                             // 16-byte loads of a thread in one sweep
+constexpr int kSweep = kThreads * 4 * kVecs;         // logits of one sweep: 16384
+constexpr int kGroups = kThreads / 8;                // groups of eight lanes, for the first threshold
+constexpr int kCandidates = 2048;
+constexpr int kMaxSegments = 16;
+constexpr int kMinSegment = 4096;
+constexpr int kTargetGroups = 512;
+static_assert(kGroups == 64, "one wave ranks the groups' maxima");
+static_assert(kGroups >= RBN_TOP_MAX, "the top-th largest group maximum bounds the top-th largest logit");
 
 // Orders logits by value, then by the lower index, in one 64-bit number: the value's bits made
 // monotonic (NaN below everything, -0 equal to +0) above the complement of the index.
@@ -14,88 +23,260 @@ __device__ __forceinline__ uint64_t order_key(float x, unsigned index) {
     if (x != x) u = 0;
     return ((uint64_t)u << 32) | (uint32_t)~index;
 }
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const unsigned u = (unsigned)(key >> 32);
+    return u == 0 ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int key_index(uint64_t key) { return (int)~(uint32_t)key; }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)v, off);
-        v = o > v ? o : v;
-    }
-    return v;
+template <int CTRL>
+__device__ __forceinline__ float lane_max(float v) {
+    const int i = __float_as_int(v);
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false)));
 }
 
-// (max, sum of exp(x - max), sum of (x - max) exp(x - max)) of two disjoint sets of logits.
+// (max, sum of exp(x - max), sum of (x - max) exp(x - max)) of a set of logits.
 struct Stat {
     float m, s, w;
 };
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float m = a.m > b.m || a.m != a.m ? a.m : b.m;
-    if (m == -INFINITY) return Stat{m, 0.0f, 0.0f};
-    // a part that vanishes against the other (one of nothing but -inf among them) adds nothing, not 0 * -inf
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return Stat{m, a.s + b.s, 0.0f};  // nothing but -inf (s = 0) or NaN (s = NaN)
+    // a part that vanishes against the other (one of nothing but -inf among them) adds nothing, not 0 * -inf;
+    // a NaN in its sum stays
     const float da = a.m - m, db = b.m - m, ca = expf(da), cb = expf(db);
     return Stat{m, a.s * ca + b.s * cb,
                 (ca == 0.0f ? 0.0f : ca * (a.w + da * a.s)) + (cb == 0.0f ? 0.0f : cb * (b.w + db * b.s))};
 }
 
-// One workgroup per row.
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(const float *__restrict__ logits, int vocab, size_t pitch,
-                                                            const int32_t *__restrict__ target, int top,
-                                                            float *__restrict__ logprob, float *__restrict__ entropy,
-                                                            int32_t *__restrict__ top_token,
-                                                            float *__restrict__ top_logprob) {
-    __shared__ Stat s_stat[kWaves];
-    __shared__ uint64_t s_key[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t r = blockIdx.x;
-    const float *x = logits + r * pitch;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int i = tid; i < vocab; i += kThreads) {
-        m = fmaxf(m, x[i]);
-        nan |= x[i] != x[i];
+// The largest `top` of the n keys in cand, sorted, to out: each key's place is the number of larger ones
+// (keys differ, their indices do).
+__device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, int top, uint64_t *out) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t key = cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += cand[j] > key;
+        if (rank < top) out[rank] = key;
     }
-    Stat st{nan ? NAN : m, 0.0f, 0.0f};
-    if (m != -INFINITY)
-        for (int i = tid; i < vocab; i += kThreads) {
-            const float d = x[i] - m, e = expf(d);
-            st.s += e;
-            st.w += e > 0.0f || e != e ? e * d : 0.0f;
+}
+
+// A row is one segment, or a few that workgroups share if there are few rows; the last workgroup of a row
+// to finish joins them (in the order of the segments).  One pass over the logits:
+//  * 16-byte loads, eight in flight per thread; the exponentials' running maximum per thread.
+//  * The top alternatives: the first sweep is held in registers; the top-th largest of the maxima of 64 groups of eight
+//    lanes bounds the top-th largest logit from below, and only logits at or above it (typically no more
+//    than twice `top`) go to a list in LDS, which is ranked by counting.  Later sweeps add what exceeds the
+//    list's last entry (their indices are higher, so equals lose).
+//  * Where the list overflows (many equal logits at the bound) or comes out short (NaN), the segment's
+//    alternatives are found one by one instead, each a pass over the segment.
+// Bound by the reading of the logits; with few rows by latency.
+__global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__restrict__ logits, int vocab, size_t pitch,
+                                                               int segments, int seg_len,
+                                                               const int32_t *__restrict__ target, int top,
+                                                               float *__restrict__ logprob, float *__restrict__ entropy,
+                                                               int32_t *__restrict__ top_token,
+                                                               float *__restrict__ top_logprob, char *parts,
+                                                               unsigned *__restrict__ tickets) {
+    __shared__ uint64_t s_cand[kCandidates];
+    __shared__ uint64_t s_top[RBN_TOP_MAX];
+    __shared__ Stat s_stat[kWaves];
+    __shared__ uint64_t s_best[kWaves];
+    __shared__ float s_group[kGroups];
+    __shared__ int s_count, s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t r = blockIdx.x / segments;
+    const int seg = blockIdx.x % segments;
+    const float *x = logits + r * pitch;
+    const int lo = seg * seg_len, hi = min(lo + seg_len, vocab), n = hi - lo;
+
+    // up to three logits before the first 16-byte boundary and behind the last: a thread each
+    const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / 4));
+    const int vecs = (n - head) / 4, tail = n - head - 4 * vecs;
+    const int vec_lo = lo + head, tail_lo = vec_lo + 4 * vecs;
+    const int sweeps = max(1, (vecs + kThreads * kVecs - 1) / (kThreads * kVecs));
+
+    Stat st{-INFINITY, 0.0f, 0.0f};
+    const int want = min(top, n);
+    bool slow = false;
+    int held = 0;             // entries of s_top
+    float bound = -INFINITY;  // value of the last of `want` entries
+    for (int sweep = 0; sweep < sweeps; ++sweep) {
+        float4 v[kVecs];
+        const int v0 = sweep * kThreads * kVecs + tid;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int k = v0 + j * kThreads;
+            v[j] = k < vecs ? *reinterpret_cast<const float4 *>(x + vec_lo + 4 * (size_t)k)
+                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         }
+        int extra = -1;  // this thread's logit outside the 16-byte part
+        if (sweep == 0 && tid < head) extra = lo + tid;
+        if (sweep == sweeps - 1 && tid >= 4 && tid < 4 + tail) extra = tail_lo + tid - 4;
+        const float xe = extra >= 0 ? x[extra] : -INFINITY;
+
+        float m = xe;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) m = fmaxf(fmaxf(fmaxf(m, v[j].x), fmaxf(v[j].y, v[j].z)), v[j].w);
+        const float here = fmaxf(m, -INFINITY);  // (not NaN)
+        if (here > st.m) {
+            // the old sums at the new maximum; w counts from the maximum too
+            const float d = st.m - here, c = expf(d);
+            st.w = c == 0.0f ? 0.0f : c * (st.w + d * st.s);
+            st.s *= c;
+            st.m = here;
+        }
+        const float ref = st.m == -INFINITY ? 0.0f : st.m;
+        auto add = [&](float a) {
+            const float d = a - ref, e = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
+            st.s += e;
+            st.w += e * fmaxf(d, -1e4f);  // e = 0 there; keeps 0 * -inf out
+        };
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) add(v[j].x), add(v[j].y), add(v[j].z), add(v[j].w);
+        add(xe);
+        if (top == 0 || slow) continue;
+
+        bool first = sweep == 0;
+        if (first) {
+            float gm = lane_max<0xB1>(here);  // quad_perm [1,0,3,2]
+            gm = lane_max<0x4E>(gm);          // quad_perm [2,3,0,1]
+            gm = lane_max<0x141>(gm);         // row_half_mirror: the other four of the eight
+            if ((lane & 7) == 0) s_group[tid >> 3] = gm;
+            if (tid == 0) s_count = 0;
+            __syncthreads();
+            // every wave ranks the 64 maxima (equals by their place)
+            const float g = s_group[lane];
+            int rank = 0;
+            for (int j = 0; j < kGroups; ++j) {
+                const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j));
+                rank += o > g || (o == g && j < lane);
+            }
+            const unsigned long long at = __ballot(rank == want - 1);
+            bound = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), (int)__builtin_ctzll(at)));
+        } else {
+            if (tid < held) s_cand[tid] = s_top[tid];
+            if (tid == 0) s_count = held;
+            __syncthreads();
+        }
+        if (first ? here >= bound : here > bound) {
+            auto take = [&](float a, int i) {
+                if (first ? a >= bound : a > bound) {
+                    const int at = atomicAdd(&s_count, 1);
+                    if (at < kCandidates) s_cand[at] = order_key(a, (unsigned)i);
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j) {
+                const int k = v0 + j * kThreads, i = vec_lo + 4 * k;
+                if (k < vecs) take(v[j].x, i), take(v[j].y, i + 1), take(v[j].z, i + 2), take(v[j].w, i + 3);
+            }
+            if (extra >= 0) take(xe, extra);
+        }
+        __syncthreads();
+        const int found = s_count;
+        const int so_far = min(n, (sweep == sweeps - 1 ? n : head + 4 * kThreads * kVecs * (sweep + 1)));
+        if (found > kCandidates || found < min(want, so_far)) {
+            slow = true;
+        } else if (first || found > held) {
+            rank_keys(s_cand, found, want, s_top);
+            held = min(found, want);
+            __syncthreads();
+            bound = held == want ? key_value(s_top[want - 1]) : -INFINITY;
+        }
+        __syncthreads();
+    }
+    if (slow) {
+        uint64_t below = ~0ull;
+        for (int j = 0; j < want; ++j) {
+            uint64_t best = 0;
+            for (int i = lo + tid; i < hi; i += kThreads) {
+                const uint64_t k = order_key(x[i], (unsigned)i);
+                if (k < below && k > best) best = k;
+            }
+            for (int off = 32; off > 0; off >>= 1) {
+                const uint64_t o = __shfl_xor((unsigned long long)best, off);
+                best = o > best ? o : best;
+            }
+            if (lane == 0) s_best[wave] = best;
+            __syncthreads();
+            best = s_best[0];
+            for (int w = 1; w < kWaves; ++w) best = s_best[w] > best ? s_best[w] : best;
+            if (tid == 0) s_top[j] = best;
+            below = best;
+            __syncthreads();
+        }
+    }
+
     for (int off = 32; off > 0; off >>= 1)
         st = join(st, Stat{__shfl_xor(st.m, off), __shfl_xor(st.s, off), __shfl_xor(st.w, off)});
     if (lane == 0) s_stat[wave] = st;
     __syncthreads();
     st = s_stat[0];
     for (int w = 1; w < kWaves; ++w) st = join(st, s_stat[w]);
-    const float log_s = logf(st.s);
-    const bool none = st.m == -INFINITY;  // nothing but -inf
-    auto lp = [&](float v) { return none ? -INFINITY : (v - st.m) - log_s; };
-    if (tid == 0) {
-        if (logprob) {
-            const int y = target[r];
-            logprob[r] = y >= 0 && y < vocab ? lp(x[y]) : 0.0f;
-        }
-        if (entropy) entropy[r] = none ? 0.0f : log_s - st.w / st.s;
-    }
-    uint64_t below = ~0ull;
-    for (int j = 0; j < top; ++j) {
-        uint64_t best = 0;
-        for (int i = tid; i < vocab; i += kThreads) {
-            const uint64_t k = order_key(x[i], (unsigned)i);
-            if (k < below && k > best) best = k;
-        }
-        best = wave_max_u64(best);
-        if (lane == 0) s_key[wave] = best;
-        __syncthreads();
-        best = s_key[0];
-        for (int w = 1; w < kWaves; ++w) best = s_key[w] > best ? s_key[w] : best;
+    int entries = want;
+
+    if (segments > 1) {
+        // partial result of a segment: keys (padded with 0, which is below every key), then the sums
+        constexpr size_t kPart = RBN_TOP_MAX * 8 + 16;
+        char *mine = parts + (size_t)blockIdx.x * kPart;
+        if (tid < RBN_TOP_MAX)
+            __hip_atomic_store(reinterpret_cast<uint64_t *>(mine) + tid, tid < want ? s_top[tid] : 0ull, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        float *ms = reinterpret_cast<float *>(mine + RBN_TOP_MAX * 8);
+        if (tid < 3)
+            __hip_atomic_store(ms + tid, tid == 0 ? st.m : tid == 1 ? st.s : st.w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // published once the stores have completed (vmcnt(0): this wave's, the barrier: everybody's)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (tid == 0) {
-            const int i = j < vocab ? (int)~(uint32_t)best : -1;
-            top_token[r * top + j] = i;
-            top_logprob[r * top + j] = i >= 0 ? lp(x[i]) : -INFINITY;
+            const int is_last = atomicAdd(&tickets[r], 1u) == (unsigned)segments - 1;
+            if (is_last) atomicExch(&tickets[r], 0u);  // ready for the next launch
+            s_last = is_last;
         }
-        below = best;
+        __syncthreads();
+        if (!s_last) return;
+        const char *all = parts + r * segments * kPart;
+        static_assert(kMaxSegments * RBN_TOP_MAX <= kThreads, "one thread per key of a partial result");
+        if (tid < segments * RBN_TOP_MAX) {
+            const int p = tid / RBN_TOP_MAX, j = tid % RBN_TOP_MAX;
+            s_cand[tid] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(all + p * kPart) + j, __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+        }
+        auto stat_of = [&](int p) {
+            const float *f = reinterpret_cast<const float *>(all + p * kPart + RBN_TOP_MAX * 8);
+            return Stat{__hip_atomic_load(f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                        __hip_atomic_load(f + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                        __hip_atomic_load(f + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
+        };
+        st = stat_of(0);
+        for (int p = 1; p < segments; ++p) st = join(st, stat_of(p));
+        __syncthreads();
+        entries = min(top, vocab);
+        if (tid < segments * RBN_TOP_MAX && s_cand[tid] != 0) {
+            const uint64_t key = s_cand[tid];
+            int rank = 0;
+            for (int p = 0; p < segments; ++p)
+                for (int j = 0; j < top; ++j) rank += s_cand[p * RBN_TOP_MAX + j] > key;
+            if (rank < entries) s_top[rank] = key;
+        }
+        __syncthreads();
     }
+
+    const float log_s = logf(st.s);
+    const bool none = st.m == -INFINITY && st.s == 0.0f;  // nothing but -inf
+    auto lp = [&](float v) { return none ? -INFINITY : (v - st.m) - log_s; };
+    if (tid < top) {
+        const bool there = tid < entries;
+        const uint64_t key = there ? s_top[tid] : 0;
+        top_token[r * top + tid] = there ? key_index(key) : -1;
+        top_logprob[r * top + tid] = there ? lp(key_value(key)) : -INFINITY;
+    }
+    if (tid == 64 && logprob) {
+        const int y = target[r];
+        logprob[r] = y >= 0 && y < vocab ? lp(x[y]) : 0.0f;
+    }
+    if (tid == 128 && entropy) entropy[r] = none ? 0.0f : log_s - st.w / st.s;
 }
 
 }  // namespace
@@ -115,8 +296,18 @@ int rbn_token_logprobs_f32(rbn_ctx *ctx, const float *d_logits, uint64_t rows, u
     RBN_REQUIRE((d_logprob == nullptr) == (d_target == nullptr), "d_logprob and d_target go together");
     RBN_REQUIRE(top == 0 || (d_top_token && d_top_logprob), "top needs d_top_token and d_top_logprob");
     RBN_ENTER(ctx);
-    logprobs_kernel<<<dim3((unsigned)rows), dim3(kThreads), 0, ctx->stream>>>(
-        d_logits, (int)vocab, (size_t)pitch, d_target, (int)top, d_logprob, d_entropy, d_top_token, d_top_logprob);
+    // few rows: workgroups share a row, as long as each has enough to read
+    uint64_t segments = kTargetGroups / rows;
+    const uint64_t most = vocab / kMinSegment;
+    segments = segments < most ? segments : most;
+    segments = segments < kMaxSegments ? segments : kMaxSegments;
+    segments = segments > 1 ? segments : 1;
+    static_assert(kTargetGroups / 2 <= RBN_SPLITK_GROUPS, "a ticket for every row that is shared");
+    const uint64_t seg_len = (vocab + segments - 1) / segments;
+    segments = (vocab + seg_len - 1) / seg_len;
+    logprobs_kernel<<<dim3((unsigned)(rows * segments)), dim3(kThreads), 0, ctx->stream>>>(
+        d_logits, (int)vocab, (size_t)pitch, (int)segments, (int)seg_len, d_target, (int)top, d_logprob, d_entropy,
+        d_top_token, d_top_logprob, (char *)ctx->splitk_partials, ctx->splitk_tickets);
     RBN_HIP(hipGetLastError());
     return RBN_OK;
 }
