@@ -50,11 +50,33 @@ __device__ __forceinline__ float other_half(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // row_ror:8
 }
 
+// Sum over the wave, and the inclusive prefix sum, on the DPP path; all lanes must be active.
+template <int CTRL, int ROWMASK>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWMASK, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan_i(int v) {
+    v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+    v = dpp_add<0x112, 0xf>(v);  // row_shr:2
+    v = dpp_add<0x114, 0xf>(v);  // row_shr:4
+    v = dpp_add<0x118, 0xf>(v);  // row_shr:8
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast15
+    return dpp_add<0x143, 0xc>(v);  // row_bcast31
+}
+__device__ __forceinline__ int wave_sum_i(int v) { return __builtin_amdgcn_readlane(wave_scan_i(v), 63); }
+
 __device__ __forceinline__ float load_agent(const float *p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void store_agent(float *p, float v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_agent(float *p, v4f v) {  // 8-byte aligned
+    unsigned long long *to = reinterpret_cast<unsigned long long *>(p);
+    typedef unsigned long long v2q __attribute__((ext_vector_type(2)));
+    const v2q w = __builtin_bit_cast(v2q, v);
+    __hip_atomic_store(to, w.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(to + 1, w.y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Power of two at or below |v| (exponent clamped to the normal range), as an exponent.
@@ -73,333 +95,469 @@ __device__ __forceinline__ int exponent_of(float v) {
 //    (slot e of lane group g is key 16 (e/4) + 4 g + e%4; V's layout follows).
 //  * The running maximum is shared by the four lanes of a column and moves only when a score exceeds it
 //    by 8 (powers of two): the usual block costs no cross-lane step.  Sums are per lane until the end.
-//  * The blocks of an item (token or unit, K/V head, up to 8 NT columns) go round the 4 * splits
-//    waves of its workgroups; the last workgroup of an item to finish joins the partial results in
-//    a fixed order.  Bound by the reading of the codes.
+//  * The blocks of an item (token or unit, K/V head, up to 8 NT columns) go round the waves of the
+//    workgroups that share it.  How many share is decided on the device, where the lengths are: a share is
+//    what gives kTargetGroups shares in all, so that rows of any mix of lengths fill the chip evenly.
+//    The last workgroup of an item to finish joins the partial results in a fixed order.  Bound by the reading of the codes.
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
-constexpr int kMinBlocksPerWave = 2;  // before another workgroup shares an item
-constexpr int kTargetGroups = 4096;
+constexpr int kMinShare = 8;          // blocks a workgroup takes at least before another shares the item
+constexpr int kTargetGroups = 1536;   // workgroups that share the batch's blocks evenly
+constexpr int kMaxShares = 64;        // one lane for each when they are joined
+constexpr int kMostItems = 2048;      // more items fill the chip without sharing
 constexpr int kFewColumns = 16;
 
 // floats of one split's partial result: columns x (out, max, sum)
 template <int HD, int NT>
 constexpr int partial_floats() {
-    return 8 * NT * (HD + 2);
+    return 8 * NT * (HD + 2);  // outputs by column, then maxima, then sums
 }
+static_assert(kMostItems <= RBN_ATTENTION_ITEMS, "a ticket for every item that is shared");
 
 template <int FMT, int HD, int NT, bool PER_TOKEN>
 __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_token_kernel(
-    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int splits, int max_columns,
-    float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int tiles, int max_shares,
+    int max_columns, float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 32;   // k steps of the scores
     constexpr int DT = HD / 16;   // tiles of dimensions of the output
     constexpr int LD = HD / 32;   // 16-byte loads per lane of 32 keys, K and V each
     constexpr int kPitch = HD + 8;
+    constexpr int kTile = kKvBlock * HD;
     __shared__ __attribute__((aligned(16))) float s_o[kTokenWaves][8 * NT][HD];
     __shared__ __attribute__((aligned(16))) _Float16 s_open[kKvBlock * kPitch];
+    __shared__ v8h s_q[NT][KK][64];
     __shared__ float s_m[kTokenWaves][8 * NT], s_l[kTokenWaves][8 * NT];
+    __shared__ float s_weight[8 * NT][kMaxShares], s_den[8 * NT];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int c16 = lane & 15, c8 = lane & 7, g = lane >> 4;
     const int group = heads / l.kv_heads;
-    const int split = blockIdx.x % splits, item = blockIdx.x / splits, kvh = item % l.kv_heads, u = item / l.kv_heads;
-
-    // the item's tokens: `first` .. `first + n`, at positions pos .. of `row`
-    int row, first, n, pos, len;
-    if (PER_TOKEN) {
-        first = u;
-        if (u >= min(b.count[0], b.max_tokens)) return;
-        n = 1;
-        row = b.row[u];
-        pos = b.pos[u];
-        if (row < 0 || row >= t.rows) pos = -1;
+    // ---- this workgroup's task: an item (token or unit u, K/V head, tile of columns) and a share of its blocks
+    int row, first, n, pos;  // the item's tokens `first` .. `first + n` at positions pos .. of `row`
+    int u, split = 0, shares = 1;
+    const int each = l.kv_heads * tiles, rest = blockIdx.x % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
+    if (max_shares > 1) {
+        // Every wave deals out the whole batch for itself, 64 tokens (units) at a time: the blocks of all give the
+        // size of a share, and a running sum of the shares tells whose turn blockIdx.x is.  One trip to
+        // memory for up to 64 tokens, no barrier, and no idle workgroups between the busy ones.
+        const int count = min(b.count[PER_TOKEN ? 0 : 1], b.max_tokens), limit = PER_TOKEN ? b.max_tokens : count;
+        int my_row = -1, my_pos = -1, blocks = 0;
+        auto look = [&](int i) {
+            const int at = i >= limit ? -1 : PER_TOKEN ? i : b.unit[i];
+            const bool in = at >= 0 && at < b.max_tokens;
+            my_row = in ? b.row[at] : -1;
+            my_pos = in ? b.pos[at] : -1;
+            blocks = my_pos >= 0 && my_pos < t.max_blocks * kKvBlock ? my_pos / kKvBlock + 1 : 1;
+            if (i >= count) blocks = 0;
+            // rows of the other kernel get no turn
+            if (!PER_TOKEN && blocks > 0 && my_row >= 0 && my_row < t.rows &&
+                ((int64_t)b.start[my_row + 1] - b.start[my_row]) * group > max_columns)
+                blocks = 0;
+        };
+        int64_t all = 0;
+        for (int base = 0; base < limit; base += 64) {
+            look(base + lane);
+            all += wave_sum_i(blocks);
+        }
+        const int share = (int)max((int64_t)kMinShare, (all * each + kTargetGroups - 1) / kTargetGroups);
+        int turn = blockIdx.x / each;  // counts down to the item
+        for (int base = 0;; base += 64) {
+            if (base >= limit) return;  // behind the last share
+            if (limit > 64) look(base + lane);
+            const int mine = min(max_shares, (blocks + share - 1) / share);
+            const int upto = wave_scan_i(mine);
+            const unsigned long long behind = __ballot(turn < upto);
+            if (behind) {
+                const int owner = (int)__builtin_ctzll(behind);
+                u = base + owner;
+                row = __builtin_amdgcn_readlane(my_row, owner);
+                pos = __builtin_amdgcn_readlane(my_pos, owner);
+                shares = __builtin_amdgcn_readlane(mine, owner);
+                split = turn - (__builtin_amdgcn_readlane(upto, owner) - shares);
+                break;
+            }
+            turn -= __builtin_amdgcn_readlane(upto, 63);
+        }
     } else {
+        u = blockIdx.x / each;
+        if (u >= min(b.count[PER_TOKEN ? 0 : 1], b.max_tokens)) return;
+        if (PER_TOKEN) {
+            row = b.row[u];
+            pos = b.pos[u];
+        }
+    }
+    u = __builtin_amdgcn_readfirstlane(u);
+    first = u;
+    n = 1;
+    if (!PER_TOKEN) {
         const KvUnit unit = kv_unit(t, b, u, flags);
-        if (unit.n == 0 || unit.row_n * group > max_columns) return;
-        first = unit.first;
-        n = unit.n;
+        if (unit.n == 0 || unit.row_n * group > max_columns) return;  // (the other kernel's)
+        first = __builtin_amdgcn_readfirstlane(unit.first);
+        n = __builtin_amdgcn_readfirstlane(unit.n);
         row = unit.row;
         pos = unit.pos;
     }
-    len = pos >= 0 ? min(t.len[row], t.max_blocks * kKvBlock) : 0;
-    if (pos < 0 || pos + n > len) {
+    row = __builtin_amdgcn_readfirstlane(row);
+    pos = __builtin_amdgcn_readfirstlane(pos);
+    const int cols = n * group;
+    if (cg * 8 * NT >= cols) return;
+    if (row < 0 || row >= t.rows || pos < 0 || pos + n > t.max_blocks * kKvBlock) {
         if (tid == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
         return;
     }
-    const int cols = n * group;
-    const int nblocks = (pos + n - 1) / kKvBlock + 1, full_blocks = min(len / kKvBlock, nblocks);
+    const int nblocks = (pos + n - 1) / kKvBlock + 1;
+    const int stride = shares * kTokenWaves, w0 = split * kTokenWaves + wave;
 
-    // More columns than the grid's z covers (only if the host's bound was too low): the item's first
-    // workgroup does the rest alone.
-    for (int cg = blockIdx.y; cg * 8 * NT < cols; cg += gridDim.y) {
-        int shares = min(splits, (nblocks + kTokenWaves * kMinBlocksPerWave - 1) / (kTokenWaves * kMinBlocksPerWave));
-        if (cg != (int)blockIdx.y) shares = 1;
-        if (split >= shares) continue;
-        const int stride = shares * kTokenWaves, w0 = split * kTokenWaves + wave;
-
-        // Q^T operand and what belongs to a column
-        v8h qf[NT][KK];
-        float col_scale[NT];   // 2^e log2(e) / sqrt(hd): raw score x K scale x this is an exponent of two
-        int col_pos[NT];
+    float x[NT][KK][8];  // this lane's part of its columns of q
+    auto load_q = [&]() {
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
-            const int c = min((cg * NT + ct) * 8 + c8, cols - 1);
+            const int c = min((cg * NT + ct) * 8 + c8, n * group - 1);
             const int token = c / group;
             const float *src = q + ((size_t)(first + token) * heads + kvh * group + (c - token * group)) * HD + 8 * g;
-            col_pos[ct] = pos + token;
-            float x[KK][8], m = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                const float4 lo4 = *reinterpret_cast<const float4 *>(src + 32 * kk);
-                const float4 hi4 = *reinterpret_cast<const float4 *>(src + 32 * kk + 4);
-                x[kk][0] = lo4.x, x[kk][1] = lo4.y, x[kk][2] = lo4.z, x[kk][3] = lo4.w;
-                x[kk][4] = hi4.x, x[kk][5] = hi4.y, x[kk][6] = hi4.z, x[kk][7] = hi4.w;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[kk][e]));
+                const float4 a = *reinterpret_cast<const float4 *>(src + 32 * kk);
+                const float4 z = *reinterpret_cast<const float4 *>(src + 32 * kk + 4);
+                x[ct][kk][0] = a.x, x[ct][kk][1] = a.y, x[ct][kk][2] = a.z, x[ct][kk][3] = a.w;
+                x[ct][kk][4] = z.x, x[ct][kk][5] = z.y, x[ct][kk][6] = z.z, x[ct][kk][7] = z.w;
             }
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const int ex = exponent_of(m);
-            col_scale[ct] = ldexpf(HD == 128 ? kLog2eBySqrt128 : kLog2eBySqrt64, ex);
+        }
+    };
+    // pages of the wave's first 64 blocks and the row's length; the unfinished block has no page
+    int page = -1;
+    if (w0 + lane * stride < nblocks) page = kv_page(t, row, w0 + lane * stride);
+    const int len = __builtin_amdgcn_readfirstlane(min(t.len[row], t.max_blocks * kKvBlock));
+    load_q();
+    if (pos + n > len) {
+        if (tid == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+        return;
+    }
+    const int full_blocks = min(len / kKvBlock, nblocks);
+    const int mine = full_blocks > w0 ? (full_blocks - w0 + stride - 1) / stride : 0;
+
+    // Codes of a block: LD 16-byte loads each for K and V (an invalid page loads page 0 and is skipped).
+    v4u kc[LD], vc[LD];
+    auto load = [&](v4u (&to)[LD], const uint8_t *codes, int pg) {
+        const v4u *src =
+            reinterpret_cast<const v4u *>(codes + ((size_t)max(pg, 0) * l.kv_heads + kvh) * (kKvBlock * HD)) + lane;
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
+        for (int j = 0; j < LD; ++j) to[j] = src[64 * j];
+    };
+    float ks = 0.0f, vs = 0.0f;
+    auto load_scales = [&](int steps) {
+        if (lane < steps) {
+            const size_t ph = (size_t)max(page, 0) * l.kv_heads + kvh;
+            ks = l.k_scale[ph];
+            vs = l.v_scale[ph];
+            if (page < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+        }
+    };
+    if (mine > 0) {
+        load(kc, l.k, __builtin_amdgcn_readlane(page, 0));
+        load(vc, l.v, __builtin_amdgcn_readlane(page, 0));
+        load_scales(min(64, mine));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // Q^T operand and what belongs to a column.  A wave prepares every kTokenWaves-th k step for all.
+    v8h qf[NT][KK];
+    float col_scale[NT];   // 2^e log2(e) / sqrt(hd): raw score x K scale x this is an exponent of two
+    int col_pos[NT];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+        col_pos[ct] = pos + min((cg * NT + ct) * 8 + c8, cols - 1) / group;
+        float m = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[ct][kk][e]));
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const int ex = exponent_of(m);
+        col_scale[ct] = ldexpf(HD == 128 ? kLog2eBySqrt128 : kLog2eBySqrt64, ex);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+            if (wave == kk % kTokenWaves) {
+                v8h z;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float v = ldexpf(x[kk][e], -ex);
-                    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
-                    qf[ct][kk][e] = c16 < 8 ? hi : lo;
+                    const float v = ldexpf(x[ct][kk][e], -ex);
+                    const float hi = (float)(_Float16)v;
+                    z[e] = (_Float16)(c16 < 8 ? hi : v - hi);
                 }
-        }
+                s_q[ct][kk][lane] = z;
+            }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) qf[ct][kk] = s_q[ct][kk][lane];
 
-        float run_max[NT], run_sum[NT];
-        v4f o[NT][DT];
+    float run_max[NT], run_sum[NT];
+    v4f o[NT][DT];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+        run_max[ct] = -INFINITY;
+        run_sum[ct] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[ct][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // Scores of 32 keys from t0 on (tile a, register r: key 16 a + 4 g + r), their softmax and P.V.
+    auto attend = [&](const v4f (&s)[NT][2], auto value, float kscale, float vscale, int t0) {
+        const bool masked = t0 + kKvBlock - 1 > pos;
+        v8h pf[NT];
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
-            run_max[ct] = -INFINITY;
-            run_sum[ct] = 0.0f;
+            const float f = kscale * col_scale[ct];
+            float x[8], m = -INFINITY;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[ct][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = 0; e < 8; ++e) {
+                x[e] = s[ct][e >> 2][e & 3];
+                x[e] = (x[e] + other_half(x[e])) * f;
+                if (masked) x[e] = t0 + 16 * (e >> 2) + 4 * g + (e & 3) <= col_pos[ct] ? x[e] : -INFINITY;
+                m = fmaxf(m, x[e]);
+            }
+            if (__any(m > run_max[ct] + 8.0f)) {
+                m = fmaxf(m, __shfl_xor(m, 16));
+                m = fmaxf(m, __shfl_xor(m, 32));
+                const float top = fmaxf(run_max[ct], m);
+                const float corr = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max[ct] - top);
+                run_max[ct] = top;
+                run_sum[ct] *= corr;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[ct][d] *= corr;
+            }
+            const float ref = run_max[ct] == -INFINITY ? 0.0f : run_max[ct];  // nothing seen yet: p = 0
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __builtin_amdgcn_exp2f(x[e] - ref);
+                run_sum[ct] += p;
+                const _Float16 hi = (_Float16)p, lo = (_Float16)(p - (float)hi);
+                pf[ct][e] = c16 < 8 ? hi : lo;
+            }
         }
-        // Scores of 32 keys from t0 on (tile a, register r: key 16 a + 4 g + r), their softmax and P.V.
-        auto attend = [&](const v4f (&s)[NT][2], auto value, float kscale, float vscale, int t0) {
-            const bool masked = t0 + kKvBlock - 1 > pos;
-            v8h pf[NT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const v8h vf = value(d);
 #pragma unroll
             for (int ct = 0; ct < NT; ++ct) {
-                const float f = kscale * col_scale[ct];
-                float x[8], m = -INFINITY;
+                const v4f z = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = s[ct][e >> 2][e & 3];
-                    x[e] = (x[e] + other_half(x[e])) * f;
-                    if (masked) x[e] = t0 + 16 * (e >> 2) + 4 * g + (e & 3) <= col_pos[ct] ? x[e] : -INFINITY;
-                    m = fmaxf(m, x[e]);
-                }
-                if (__any(m > run_max[ct] + 8.0f)) {
-                    m = fmaxf(m, __shfl_xor(m, 16));
-                    m = fmaxf(m, __shfl_xor(m, 32));
-                    const float top = fmaxf(run_max[ct], m);
-                    const float corr = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max[ct] - top);
-                    run_max[ct] = top;
-                    run_sum[ct] *= corr;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[ct][d] *= corr;
-                }
-                const float ref = run_max[ct] == -INFINITY ? 0.0f : run_max[ct];  // nothing seen yet: p = 0
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(x[e] - ref);
-                    run_sum[ct] += p;
-                    const _Float16 hi = (_Float16)p, lo = (_Float16)(p - (float)hi);
-                    pf[ct][e] = c16 < 8 ? hi : lo;
-                }
+                for (int r = 0; r < 4; ++r) o[ct][d][r] = fmaf(z[r], vscale, o[ct][d][r]);
             }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const v8h vf = value(d);
-#pragma unroll
-                for (int ct = 0; ct < NT; ++ct) {
-                    const v4f z = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[ct][d][r] = fmaf(z[r], vscale, o[ct][d][r]);
-                }
-            }
-        };
+        }
+    };
 
-        // full blocks: this wave's w0, w0 + stride, ...
-        const int mine = full_blocks > w0 ? (full_blocks - w0 + stride - 1) / stride : 0;
-        v4u kc[LD], vc[LD];
-        // (an invalid page loads page 0 and is skipped)
-        auto load = [&](v4u (&to)[LD], const uint8_t *codes, int page) {
-            const v4u *src =
-                reinterpret_cast<const v4u *>(codes + ((size_t)max(page, 0) * l.kv_heads + kvh) * (kKvBlock * HD)) + lane;
-#pragma unroll
-            for (int j = 0; j < LD; ++j) to[j] = src[64 * j];
-        };
-        for (int base = 0; base < mine; base += 64) {
-            // pages and scales of the next 64 blocks, one per lane
-            const int steps = min(64, mine - base);
-            int page = -1;
-            float ks = 0.0f, vs = 0.0f;
-            if (lane < steps) {
-                page = kv_page(t, row, w0 + (base + lane) * stride);
-                const size_t ph = (size_t)max(page, 0) * l.kv_heads + kvh;
-                ks = l.k_scale[ph];
-                vs = l.v_scale[ph];
-                if (page < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
-            }
+    // full blocks: this wave's w0, w0 + stride, ...
+    for (int base = 0; base < mine; base += 64) {
+        const int steps = min(64, mine - base);
+        if (base > 0) {
+            page = -1;
+            if (lane < steps) page = kv_page(t, row, w0 + (base + lane) * stride);
             load(kc, l.k, __builtin_amdgcn_readlane(page, 0));
             load(vc, l.v, __builtin_amdgcn_readlane(page, 0));
-            for (int i = 0; i < steps; ++i) {
-                const int here = __builtin_amdgcn_readlane(page, i), next = __builtin_amdgcn_readlane(page, min(i + 1, steps - 1));
-                v4f s[NT][2];
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-#pragma unroll
-                    for (int ct = 0; ct < NT; ++ct) s[ct][a] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        const v4u w = kc[a * (KK / 2) + kk / 2];
-                        const v8h kf = kk & 1 ? codes_to_f16<FMT>(w.z, w.w) : codes_to_f16<FMT>(w.x, w.y);
-#pragma unroll
-                        for (int ct = 0; ct < NT; ++ct)
-                            s[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ct][kk], s[ct][a], 0, 0, 0);
-                    }
-                }
-                load(kc, l.k, next);  // the next block's keys travel during the softmax, its values during its scores
-                if (here >= 0)
-                    attend(s,
-                           [&](int d) {
-                               const v4u w = vc[d / 2];
-                               return d & 1 ? codes_to_f16<FMT>(w.z, w.w) : codes_to_f16<FMT>(w.x, w.y);
-                           },
-                           __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), i)),
-                           __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), i)),
-                           (w0 + (base + i) * stride) * kKvBlock);
-                load(vc, l.v, next);
-            }
+            load_scales(steps);
         }
-        // the unfinished block, f16: K straight from the buffer, V transposed through LDS; rows behind
-        // the end may hold anything, so V's are zeroed (K's scores are masked)
-        if (nblocks > full_blocks && full_blocks % stride == w0) {
-            const size_t at = ((size_t)row * l.kv_heads + kvh) * kKvBlock * HD;
-            const _Float16 *ko = reinterpret_cast<const _Float16 *>(l.k_open) + at;
-            const _Float16 *vo = reinterpret_cast<const _Float16 *>(l.v_open) + at;
-            const int valid = len - full_blocks * kKvBlock;
-            v8h kf[2][KK];
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-                    kf[a][kk] = *reinterpret_cast<const v8h *>(ko + (size_t)(16 * a + c16) * HD + 32 * kk + 8 * g);
-#pragma unroll
-            for (int j = 0; j < kKvBlock * HD / 512; ++j) {
-                const int e = j * 512 + lane * 8, key = e / HD, d = e % HD;
-                v8h x = *reinterpret_cast<const v8h *>(vo + e);
-                if (key >= valid) x = v8h{0, 0, 0, 0, 0, 0, 0, 0};
-                *reinterpret_cast<v8h *>(s_open + key * kPitch + d) = x;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < steps; ++i) {
+            const int here = __builtin_amdgcn_readlane(page, i), next = __builtin_amdgcn_readlane(page, min(i + 1, steps - 1));
             v4f s[NT][2];
 #pragma unroll
-            for (int ct = 0; ct < NT; ++ct)
+            for (int a = 0; a < 2; ++a) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    s[ct][a] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int ct = 0; ct < NT; ++ct) s[ct][a] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk)
-                        s[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[a][kk], qf[ct][kk], s[ct][a], 0, 0, 0);
+                for (int kk = 0; kk < KK; ++kk) {
+                    const v4u w = kc[a * (KK / 2) + kk / 2];
+                    const v8h kf = kk & 1 ? codes_to_f16<FMT>(w.z, w.w) : codes_to_f16<FMT>(w.x, w.y);
+#pragma unroll
+                    for (int ct = 0; ct < NT; ++ct)
+                        s[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ct][kk], s[ct][a], 0, 0, 0);
                 }
-            attend(s,
-                   [&](int d) {
-                       v8h vf;
-#pragma unroll
-                       for (int e = 0; e < 8; ++e) vf[e] = s_open[(16 * (e >> 2) + 4 * g + (e & 3)) * kPitch + 16 * d + c16];
-                       return vf;
-                   },
-                   1.0f, 1.0f, full_blocks * kKvBlock);
+            }
+            load(kc, l.k, next);  // the next block's keys travel during the softmax, its values during its scores
+            if (here >= 0)
+                attend(s,
+                       [&](int d) {
+                           const v4u w = vc[d / 2];
+                           return d & 1 ? codes_to_f16<FMT>(w.z, w.w) : codes_to_f16<FMT>(w.x, w.y);
+                       },
+                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), i)),
+                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), i)),
+                       (w0 + (base + i) * stride) * kKvBlock);
+            load(vc, l.v, next);
         }
+    }
+    // the unfinished block, f16: K straight from the buffer, V transposed through LDS; rows behind
+    // the end may hold anything, so V's are zeroed (K's scores are masked)
+    if (nblocks > full_blocks && full_blocks % stride == w0) {
+        const size_t at = ((size_t)row * l.kv_heads + kvh) * kKvBlock * HD;
+        const _Float16 *ko = reinterpret_cast<const _Float16 *>(l.k_open) + at;
+        const _Float16 *vo = reinterpret_cast<const _Float16 *>(l.v_open) + at;
+        const int valid = len - full_blocks * kKvBlock;
+        v8h kf[2][KK], vx[kTile / 512];
+        const unsigned k0 = c16 * HD + 8 * g, v0 = lane * 8;
+#pragma unroll
+        for (int j = 0; j < kTile / 512; ++j) vx[j] = *reinterpret_cast<const v8h *>(vo + (v0 + j * 512));
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) kf[a][kk] = *reinterpret_cast<const v8h *>(ko + (k0 + 16 * a * HD + 32 * kk));
+        __builtin_amdgcn_sched_barrier(0);  // all on their way before the first is waited for
+#pragma unroll
+        for (int j = 0; j < kTile / 512; ++j) {
+            const int key = (v0 + j * 512) / HD, d = (v0 + j * 512) % HD;
+            if (key >= valid) vx[j] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+            *reinterpret_cast<v8h *>(s_open + key * kPitch + d) = vx[j];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        v4f s[NT][2];
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                s[ct][a] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    s[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[a][kk], qf[ct][kk], s[ct][a], 0, 0, 0);
+            }
+        attend(s,
+               [&](int d) {
+                   v8h vf;
+#pragma unroll
+                   for (int e = 0; e < 8; ++e) vf[e] = s_open[(16 * (e >> 2) + 4 * g + (e & 3)) * kPitch + 16 * d + c16];
+                   return vf;
+               },
+               1.0f, 1.0f, full_blocks * kKvBlock);
+    }
 
-        // the waves meet
+    // the waves meet
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) {
-            run_sum[ct] += __shfl_xor(run_sum[ct], 16);
-            run_sum[ct] += __shfl_xor(run_sum[ct], 32);
-            if (lane < 8) {
-                s_m[wave][ct * 8 + lane] = run_max[ct];
-                s_l[wave][ct * 8 + lane] = run_sum[ct];
+    for (int ct = 0; ct < NT; ++ct) {
+        run_sum[ct] += __shfl_xor(run_sum[ct], 16);
+        run_sum[ct] += __shfl_xor(run_sum[ct], 32);
+        if (lane < 8) {
+            s_m[wave][ct * 8 + lane] = run_max[ct];
+            s_l[wave][ct * 8 + lane] = run_sum[ct];
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            v4f z = o[ct][d];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] += other_half(z[r]);
+            if (c16 < 8) *reinterpret_cast<v4f *>(&s_o[wave][ct * 8 + c8][16 * d + 4 * g]) = z;
+        }
+    }
+    __syncthreads();
+    const int ncols = min(8 * NT, cols - cg * 8 * NT);
+    const int slot = u * each + rest;  // used by shared items only
+    float *part = partials + (size_t)slot * max_shares * partial_floats<HD, NT>();
+    auto write_out = [&](int c, int d, v4f num, float den) {
+        const int col = cg * 8 * NT + c, token = col / group;
+        const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+        *reinterpret_cast<v4f *>(out + ((size_t)(first + token) * heads + kvh * group + (col - token * group)) * HD + d) =
+            num * inv;
+    };
+    for (int i = tid; i < ncols * (HD / 4); i += kTokenThreads) {
+        const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+        float wm[kTokenWaves], wl[kTokenWaves], m = -INFINITY, den = 0.0f;
+        v4f num = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kTokenWaves; ++w) {
+            wm[w] = s_m[w][c];
+            wl[w] = s_l[w][c];
+            m = fmaxf(m, wm[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < kTokenWaves; ++w) {
+            // a wave that saw no key has sum 0; one that saw a NaN only has maximum -inf and a NaN sum
+            const float k = wm[w] == -INFINITY ? (wl[w] != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(wm[w] - m);
+            num += k * *reinterpret_cast<const v4f *>(&s_o[w][c][d]);
+            den += k * wl[w];
+        }
+        if (shares == 1) {
+            write_out(c, d, num, den);
+        } else {
+            float *p = part + (size_t)split * partial_floats<HD, NT>();
+            store_agent(p + c * HD + d, num);
+            if (d == 0) {
+                store_agent(p + 8 * NT * HD + c, m);
+                store_agent(p + 8 * NT * (HD + 1) + c, den);
             }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                v4f z = o[ct][d];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) z[r] += other_half(z[r]);
-                if (c16 < 8) *reinterpret_cast<v4f *>(&s_o[wave][ct * 8 + c8][16 * d + 4 * g]) = z;
-            }
+        }
+    }
+    if (shares > 1) {
+        // published once the stores have completed (vmcnt(0): this wave's, the barrier: everybody's)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            const int is_last = atomicAdd(&tickets[slot], 1u) == (unsigned)shares - 1;
+            if (is_last) atomicExch(&tickets[slot], 0u);  // ready for the next launch
+            s_last = is_last;
         }
         __syncthreads();
-        const int ncols = min(8 * NT, cols - cg * 8 * NT);
-        const int slot = item * gridDim.y + cg;  // used by shared items only
-        float *part = partials + (size_t)slot * splits * partial_floats<HD, NT>();
-        auto write_out = [&](int c, int d, float num, float den) {
-            const int col = cg * 8 * NT + c, token = col / group;
-            out[((size_t)(first + token) * heads + kvh * group + (col - token * group)) * HD + d] =
-                den > 0.0f || den != den ? num / den : 0.0f;
-        };
-        for (int i = tid; i < ncols * HD; i += kTokenThreads) {
-            const int c = i / HD, d = i % HD;
-            float m = -INFINITY, num = 0.0f, den = 0.0f;
+        if (s_last) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            // outputs in quads; `lots` threads share one and meet in LDS.  The first loads go out before
+            // the weights are known.
+            const int quads = ncols * (HD / 4), lots = max(1, kTokenThreads / quads);
+            const int my_quad = tid % quads, my_lot = tid / quads;
+            const v4f *p0 = reinterpret_cast<const v4f *>(part) + my_quad;
+            constexpr int kAhead = 8;
+            v4f ahead[kAhead];
+            if (my_lot < lots)
 #pragma unroll
-            for (int w = 0; w < kTokenWaves; ++w) m = fmaxf(m, s_m[w][c]);
-#pragma unroll
-            for (int w = 0; w < kTokenWaves; ++w) {
-                // a wave that saw no key has sum 0; one that saw a NaN only has maximum -inf and a NaN sum
-                const float k = s_m[w][c] == -INFINITY ? (s_l[w][c] != 0.0f ? 1.0f : 0.0f)
-                                                       : __builtin_amdgcn_exp2f(s_m[w][c] - m);
-                num += k * s_o[w][c][d];
-                den += k * s_l[w][c];
-            }
-            if (shares == 1) {
-                write_out(c, d, num, den);
-            } else {
-                float *p = part + (size_t)split * partial_floats<HD, NT>() + c * (HD + 2);
-                store_agent(p + d, num);
-                if (d == 0) {
-                    store_agent(p + HD, m);
-                    store_agent(p + HD + 1, den);
+                for (int j = 0; j < kAhead; ++j)
+                    ahead[j] = p0[(size_t)min(my_lot + j * lots, shares - 1) * (partial_floats<HD, NT>() / 4)];
+            // weights: a wave per column, a lane per share
+            for (int c = wave; c < ncols; c += kTokenWaves) {
+                float pm = -INFINITY, pl = 0.0f;
+                if (lane < shares) {
+                    const float *p = part + (size_t)lane * partial_floats<HD, NT>() + 8 * NT * HD + c;
+                    pm = load_agent(p);
+                    pl = load_agent(p + 8 * NT);
                 }
-            }
-        }
-        if (shares > 1) {
-            // published once the stores have completed (vmcnt(0): this wave's, the barrier: everybody's)
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (tid == 0) {
-                const int is_last = atomicAdd(&tickets[slot], 1u) == (unsigned)shares - 1;
-                if (is_last) atomicExch(&tickets[slot], 0u);  // ready for the next launch
-                s_last = is_last;
+                float m = pm;
+                for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+                const float k = pm == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pm - m);
+                float den = k * pl;
+                for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+                s_weight[c][lane] = k;
+                if (lane == 0) s_den[c] = den;
             }
             __syncthreads();
-            if (s_last)
-                for (int i = tid; i < ncols * HD; i += kTokenThreads) {
-                    const int c = i / HD, d = i % HD;
-                    const float *p = part + c * (HD + 2);
-                    float m = -INFINITY, num = 0.0f, den = 0.0f;
-                    for (int sp = 0; sp < shares; ++sp) m = fmaxf(m, load_agent(p + (size_t)sp * partial_floats<HD, NT>() + HD));
-                    for (int sp = 0; sp < shares; ++sp) {
-                        const float *ps = p + (size_t)sp * partial_floats<HD, NT>();
-                        const float pm = load_agent(ps + HD), pl = load_agent(ps + HD + 1);
-                        const float k = pm == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pm - m);
-                        num += k * load_agent(ps + d);
-                        den += k * pl;
-                    }
-                    write_out(c, d, num, den);
+            v4f *s_acc = reinterpret_cast<v4f *>(&s_o[0][0][0]);
+            for (int i = tid; i < quads * lots; i += kTokenThreads) {
+                const int quad = i % quads, lot = i / quads, c = quad / (HD / 4);
+                const v4f *p = reinterpret_cast<const v4f *>(part) + quad;
+                v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                auto add = [&](v4f z, int sp) {
+                    const float k = s_weight[c][sp];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[r] = fmaf(k, z[r], acc[r]);
+                };
+                int sp = lot;
+                if (i == tid) {
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        if (lot + j * lots < shares) add(ahead[j], lot + j * lots);
+                    sp += kAhead * lots;
                 }
+#pragma unroll 8
+                for (; sp < shares; sp += lots) add(p[(size_t)sp * (partial_floats<HD, NT>() / 4)], sp);
+                s_acc[i] = acc;
+            }
+            __syncthreads();
+            for (int i = tid; i < quads; i += kTokenThreads) {
+                const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+                v4f num = s_acc[i];
+                for (int lot = 1; lot < lots; ++lot) num += s_acc[lot * quads + i];
+                write_out(c, d, num, s_den[c]);
+            }
         }
-        __syncthreads();
     }
 }
 
@@ -746,19 +904,21 @@ int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const 
                     const AttentionShape &shape, float *d_out) {
     const uint64_t items = (uint64_t)(PER_TOKEN ? (unsigned)b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
     const uint64_t tiles = (shape.columns + 8 * NT - 1) / (8 * NT);
-    // Workgroups that share an item: enough to fill the chip several times over (rows differ in length, and
-    // short ones leave their share early), as far as tickets and partial results have room.
-    uint64_t splits = kTargetGroups / (items * tiles);
-    const uint64_t most = ((uint64_t)t.max_blocks + kTokenWaves * kMinBlocksPerWave - 1) / (kTokenWaves * kMinBlocksPerWave);
-    const uint64_t room = (uint64_t)RBN_SPLITK_TILES * 1024 / (items * tiles * partial_floats<HD, NT>());
-    splits = splits < most ? splits : most;
-    splits = splits < room ? splits : room;
-    if (splits < 1 || items * tiles > RBN_ATTENTION_ITEMS) splits = 1;
-    RBN_REQUIRE(items * splits < (1ull << 31), "too many tokens in rbn_attention_q8kv");
-    attention_token_kernel<FMT, HD, NT, PER_TOKEN>
-        <<<dim3((unsigned)(items * splits), (unsigned)tiles), dim3(kTokenThreads), 0, ctx->stream>>>(
-            d_q, t, b, l, shape.heads, (int)splits, shape.max_columns, (float *)ctx->splitk_partials,
-            ctx->attention_tickets, d_out, ctx->dev_flags);
+    // The most workgroups that may share an item, as far as tickets and partial results have room; how
+    // many do is decided on the device, where at most kTargetGroups shares and one rounded up for each item
+    // come out.
+    const uint64_t slots = items * tiles;
+    const uint64_t most = ((uint64_t)t.max_blocks + kMinShare - 1) / kMinShare;
+    const uint64_t room = (uint64_t)RBN_SPLITK_TILES * 1024 / (slots * partial_floats<HD, NT>());
+    uint64_t shares = most < kMaxShares ? most : kMaxShares;
+    shares = shares < room ? shares : room;
+    if (shares < 1 || slots > kMostItems) shares = 1;
+    uint64_t groups = slots * shares;
+    if (shares > 1 && groups > slots + kTargetGroups) groups = slots + kTargetGroups;
+    RBN_REQUIRE(groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
+    attention_token_kernel<FMT, HD, NT, PER_TOKEN><<<dim3((unsigned)groups), dim3(kTokenThreads), 0, ctx->stream>>>(
+        d_q, t, b, l, shape.heads, (int)tiles, (int)shares, shape.max_columns, (float *)ctx->splitk_partials,
+        ctx->attention_tickets, d_out, ctx->dev_flags);
     RBN_HIP(hipGetLastError());
     return RBN_OK;
 }
@@ -825,14 +985,13 @@ int rbn_attention_q8kv(rbn_ctx *ctx, const float *d_q, const rbn_kv_table *table
                 layer->kv_heads);
     RBN_REQUIRE(max_new > 0, "max_new of rbn_attention_q8kv is 0");
     RBN_ENTER(ctx);
-    // Rows with few columns go to the first kernel, the others to the second; where the host knows that there
-    // are only few, the second is not launched and the first takes all.
+    // One token per row: the first kernel, token by token (if a row has more after all, so are they).  Otherwise
+    // rows with few columns go to the first kernel, the others to the second.
     const uint64_t group = heads / layer->kv_heads;
-    const bool few = max_new == 1 || max_new * group <= kFewColumns;
-    AttentionShape shape{layer->head_dim, layer->format, (int)heads, max_new == 1, few ? max_new * group : kFewColumns,
-                         few ? INT32_MAX : kFewColumns};
+    AttentionShape shape{layer->head_dim, layer->format, (int)heads, max_new == 1, max_new == 1 ? group : kFewColumns,
+                         max_new == 1 ? INT32_MAX : kFewColumns};
     RBN_CHECK(launch_token(ctx, d_q, t, b, l, shape, d_out));
-    if (!few) RBN_CHECK(launch_prompt(ctx, d_q, t, b, l, shape, d_out));
+    if (max_new > 1) RBN_CHECK(launch_prompt(ctx, d_q, t, b, l, shape, d_out));
     return RBN_OK;
 }
 
