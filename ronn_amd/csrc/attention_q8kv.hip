@@ -87,6 +87,125 @@ __device__ __forceinline__ int exponent_of(float v) {
     return e < -126 ? -126 : e;
 }
 
+// ---- who does what ------------------------------------------------------------------------------
+// A workgroup's task: an entry of the batch (a token, or a unit), and a share of its blocks.
+struct Task {
+    int entry;         // -1: none
+    int split, shares; // this workgroup is number `split` of `shares`
+    int place;         // shares of the entries before this one that are shared: where the partial results go
+    KvUnit unit;       // of a token: n = 1, no row_*
+};
+
+// Deals the batch out in shares of equal size, so that rows of any mix of lengths fill the chip evenly.  Every
+// wave does it for itself: the blocks of all entries give the size of a share, and a running sum of the shares
+// tells whose turn blockIdx.x is: one trip through the batch's arrays for up to 256 entries, no barrier, no idle
+// workgroups between the busy ones.  Rows with fewer columns than min_columns or more than max_columns get no
+// turn.  `each`: workgroups with the same share of an entry; `target`: shares times `each` wanted in all (one more
+// for each entry can come out, and no more than 2 target belong to entries that are shared); least, most: blocks of
+// a share at least, while that gives no more than a workgroup per CU and beyond.  REVERSE: last entries first.
+constexpr int kComputeUnits = 256;
+constexpr int kLook = 4;  // rounds of 64 entries looked at together
+
+template <bool PER_TOKEN, bool REVERSE>
+__device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b, int group, int min_columns, int max_columns,
+                                     int each, int max_shares, int target, int least, int most, unsigned *flags) {
+    const int lane = threadIdx.x & 63;
+    const int tokens = min(b.count[0], b.max_tokens), count = PER_TOKEN ? tokens : min(b.count[1], b.max_tokens);
+    const int limit = PER_TOKEN ? b.max_tokens : count;  // (tokens are read up to the capacity: no wait for the count)
+    Task r;
+    r.entry = -1;
+    KvUnit mine[kLook];
+    int blocks[kLook];
+    auto look = [&](int base) {
+        int at[kLook], row[kLook], pos[kLook], s0[kLook], s1[kLook];
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+            const int i = base + 64 * k + lane;
+            at[k] = i >= limit ? -1 : PER_TOKEN ? i : b.unit[REVERSE ? count - 1 - i : i];
+        }
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+            const bool in = at[k] >= 0 && at[k] < b.max_tokens;
+            row[k] = in ? b.row[at[k]] : -1;
+            pos[k] = in ? b.pos[at[k]] : -1;
+        }
+        if (!PER_TOKEN) {
+#pragma unroll
+            for (int k = 0; k < kLook; ++k) {
+                const bool known = row[k] >= 0 && row[k] < t.rows;
+                s0[k] = known ? b.start[row[k]] : -1;
+                s1[k] = known ? b.start[row[k] + 1] : -1;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+            const int i = base + 64 * k + lane;
+            if (PER_TOKEN) {
+                mine[k].row = row[k];
+                mine[k].pos = pos[k];
+                blocks[k] = pos[k] >= 0 && pos[k] < t.max_blocks * kKvBlock ? pos[k] / kKvBlock + 1 : 1;
+            } else {
+                mine[k] = kv_make_unit(t, tokens, at[k], row[k], pos[k], s0[k], s1[k]);
+                if (i < count && mine[k].n == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+                const int64_t columns = mine[k].n > 0 ? (int64_t)mine[k].row_n * group : -1;
+                blocks[k] = columns >= min_columns && columns <= max_columns ? pos[k] / kKvBlock + 1 : 0;
+            }
+            if (i >= count) blocks[k] = 0;
+        }
+    };
+    int turn = blockIdx.x / each, share = INT32_MAX / 2;  // turn counts down to the entry
+    if (max_shares > 1 || limit <= 64 * kLook) {
+        int64_t all = 0;
+        for (int base = 0; base < limit; base += 64 * kLook) {
+            look(base);
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < kLook; ++k) sum += blocks[k];
+            all += wave_sum_i(sum);
+        }
+        if (all == 0) return r;
+        all *= each;
+        if (max_shares > 1)
+            share = (int)max(min((int64_t)most, max((int64_t)least, all / kComputeUnits)), (all + target - 1) / target);
+    }
+    r.place = 0;
+    for (int base = 0; base < limit; base += 64 * kLook) {
+        if (limit > 64 * kLook) look(base);
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+            const int parts = min(max_shares, (int)(((int64_t)blocks[k] + share - 1) / share));
+            const int upto = wave_scan_i(parts), shared_upto = wave_scan_i(parts > 1 ? parts : 0);
+            const unsigned long long behind = __ballot(turn < upto);
+            if (r.entry < 0 && behind) {
+                const int owner = (int)__builtin_ctzll(behind), i = base + 64 * k + owner;
+                auto of = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+                r.entry = REVERSE ? count - 1 - i : i;
+                r.shares = of(parts);
+                r.split = turn - (of(upto) - r.shares);
+                r.place += of(shared_upto) - (r.shares > 1 ? r.shares : 0);
+                r.unit.row = of(mine[k].row);
+                r.unit.pos = of(mine[k].pos);
+                if (PER_TOKEN) {
+                    r.unit.first = r.entry;
+                    r.unit.n = 1;
+                } else {
+                    r.unit.first = of(mine[k].first);
+                    r.unit.n = of(mine[k].n);
+                    r.unit.row_first = of(mine[k].row_first);
+                    r.unit.row_pos = of(mine[k].row_pos);
+                    r.unit.row_n = of(mine[k].row_n);
+                }
+            }
+            if (r.entry < 0) {
+                turn -= __builtin_amdgcn_readlane(upto, 63);
+                r.place += __builtin_amdgcn_readlane(shared_upto, 63);
+            }
+        }
+        if (r.entry >= 0) return r;
+    }
+    return r;
+}
+
 // ---- few query columns: decode steps ------------------------------------------------------------
 // S^T = K . Q^T and O^T = V^T . P^T on v_mfma_f32_16x16x32_f16, a wave on one block of 32 keys at a time.
 //  * The codes are exact in f16.  q (scaled to |q| < 2 by a power of two for each column) and the
@@ -104,10 +223,9 @@ __device__ __forceinline__ int exponent_of(float v) {
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
 // Blocks a workgroup takes at least before another shares the item: 8 while that gives no more than a
-// workgroup per CU, up to 16 beyond (1 x 1000 tokens, 20 heads: 10.9 us with 8, 12.4 with 16; 16 rows of 500 to
+// workgroup per CU, up to twice as many beyond (1 x 1000 tokens, 20 heads: 10.9 us with 8, 12.4 with 16; 16 rows of 500 to
 // 4000, 5 heads: 21.0 us with 8, 17.0 with 16).
 constexpr int kMinShare = 8;
-constexpr int kComputeUnits = 256;
 constexpr int kTargetGroups = 1536;   // workgroups that share the batch's blocks evenly
 constexpr int kMaxShares = 64;        // one lane for each when they are joined; more cost more there than they gain
 constexpr int kMostItems = 2048;      // more items fill the chip without sharing
@@ -138,75 +256,13 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int c16 = lane & 15, c8 = lane & 7, g = lane >> 4;
     const int group = heads / l.kv_heads;
-    // ---- this workgroup's task: an item (token or unit u, K/V head, tile of columns) and a share of its blocks
-    int row, first, n, pos;  // the item's tokens `first` .. `first + n` at positions pos .. of `row`
-    int u, split = 0, shares = 1;
+    // this workgroup's task: an item (token or unit, K/V head, tile of columns) and a share of its blocks
     const int each = l.kv_heads * tiles, rest = blockIdx.x % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
-    if (max_shares > 1) {
-        // Every wave deals out the whole batch for itself, 64 tokens (units) at a time: the blocks of all give the
-        // size of a share, and a running sum of the shares tells whose turn blockIdx.x is.  One trip to
-        // memory for up to 64 tokens, no barrier, and no idle workgroups between the busy ones.
-        const int count = min(b.count[PER_TOKEN ? 0 : 1], b.max_tokens), limit = PER_TOKEN ? b.max_tokens : count;
-        int my_row = -1, my_pos = -1, blocks = 0;
-        auto look = [&](int i) {
-            const int at = i >= limit ? -1 : PER_TOKEN ? i : b.unit[i];
-            const bool in = at >= 0 && at < b.max_tokens;
-            my_row = in ? b.row[at] : -1;
-            my_pos = in ? b.pos[at] : -1;
-            blocks = my_pos >= 0 && my_pos < t.max_blocks * kKvBlock ? my_pos / kKvBlock + 1 : 1;
-            if (i >= count) blocks = 0;
-            // rows of the other kernel get no turn
-            if (!PER_TOKEN && blocks > 0 && my_row >= 0 && my_row < t.rows &&
-                ((int64_t)b.start[my_row + 1] - b.start[my_row]) * group > max_columns)
-                blocks = 0;
-        };
-        int64_t all = 0;
-        for (int base = 0; base < limit; base += 64) {
-            look(base + lane);
-            all += wave_sum_i(blocks);
-        }
-        all *= each;
-        const int64_t least = min((int64_t)2 * kMinShare, max((int64_t)kMinShare, all / kComputeUnits));
-        const int share = (int)max(least, (all + kTargetGroups - 1) / kTargetGroups);
-        int turn = blockIdx.x / each;  // counts down to the item
-        for (int base = 0;; base += 64) {
-            if (base >= limit) return;  // behind the last share
-            if (limit > 64) look(base + lane);
-            const int mine = min(max_shares, (blocks + share - 1) / share);
-            const int upto = wave_scan_i(mine);
-            const unsigned long long behind = __ballot(turn < upto);
-            if (behind) {
-                const int owner = (int)__builtin_ctzll(behind);
-                u = base + owner;
-                row = __builtin_amdgcn_readlane(my_row, owner);
-                pos = __builtin_amdgcn_readlane(my_pos, owner);
-                shares = __builtin_amdgcn_readlane(mine, owner);
-                split = turn - (__builtin_amdgcn_readlane(upto, owner) - shares);
-                break;
-            }
-            turn -= __builtin_amdgcn_readlane(upto, 63);
-        }
-    } else {
-        u = blockIdx.x / each;
-        if (u >= min(b.count[PER_TOKEN ? 0 : 1], b.max_tokens)) return;
-        if (PER_TOKEN) {
-            row = b.row[u];
-            pos = b.pos[u];
-        }
-    }
-    u = __builtin_amdgcn_readfirstlane(u);
-    first = u;
-    n = 1;
-    if (!PER_TOKEN) {
-        const KvUnit unit = kv_unit(t, b, u, flags);
-        if (unit.n == 0 || unit.row_n * group > max_columns) return;  // (the other kernel's)
-        first = __builtin_amdgcn_readfirstlane(unit.first);
-        n = __builtin_amdgcn_readfirstlane(unit.n);
-        row = unit.row;
-        pos = unit.pos;
-    }
-    row = __builtin_amdgcn_readfirstlane(row);
-    pos = __builtin_amdgcn_readfirstlane(pos);
+    const Task task = deal<PER_TOKEN, false>(t, b, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
+                                             2 * kMinShare, flags);
+    if (task.entry < 0) return;
+    const int row = task.unit.row, pos = task.unit.pos, first = task.unit.first, n = task.unit.n;
+    const int split = task.split, shares = task.shares;
     const int cols = n * group;
     if (cg * 8 * NT >= cols) return;
     if (row < 0 || row >= t.rows || pos < 0 || pos + n > t.max_blocks * kKvBlock) {
@@ -464,8 +520,8 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
     }
     __syncthreads();
     const int ncols = min(8 * NT, cols - cg * 8 * NT);
-    const int slot = u * each + rest;  // used by shared items only
-    float *part = partials + (size_t)slot * max_shares * partial_floats<HD, NT>();
+    const int slot = task.entry * each + rest;  // used by shared items only
+    float *part = partials + ((size_t)task.place * each + (size_t)rest * shares) * partial_floats<HD, NT>();
     auto write_out = [&](int c, int d, v4f num, float den) {
         const int col = cg * 8 * NT + c, token = col / group;
         const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
@@ -587,8 +643,9 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
 //    [2^-4, 4) of the unit use it as it is, others move it (the store's scales span 2^-32 .. 2^9).
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 constexpr int kPromptThreads = 256;
-constexpr int kPromptTargetGroups = 512;
-constexpr int kPromptMinBlocks = 4;  // before another workgroup shares a tile's keys
+constexpr int kPromptTargetGroups = 480;  // workgroups that share the tiles' blocks evenly; partial results of twice as many fit
+constexpr int kPromptMinShare = 4;        // blocks a workgroup takes at least before another shares the tile
+constexpr int kPromptMaxShares = 16;
 
 // floats of one workgroup's partial result: four waves' registers, maxima and sums, lane by lane
 template <int HD>
@@ -598,7 +655,7 @@ constexpr int prompt_partial_floats() {
 
 template <int FMT, int HD>
 __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
-    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int splits, int min_columns,
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int max_shares, int min_columns,
     float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 16;   // k steps of the scores
     constexpr int NT = HD / 32;   // tiles of dimensions of the output
@@ -609,12 +666,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, g = lane >> 5;
     const int group = heads / l.kv_heads;
     const int per_unit = (group + 3) / 4;
-    const int split = blockIdx.x % splits, item = blockIdx.x / splits;
-    const int kvh = item % l.kv_heads, z = item / l.kv_heads % per_unit;
-    const int u = min(b.count[1], b.max_tokens) - 1 - item / l.kv_heads / per_unit;  // the long ones first
-    if (u < 0) return;
-    const KvUnit unit = kv_unit(t, b, u, flags);
-    if (unit.n == 0 || unit.row_n * group < min_columns) return;
+    // (the long ones first)
+    const int each = l.kv_heads * per_unit, rest = blockIdx.x % each, kvh = rest % l.kv_heads, z = rest / l.kv_heads;
+    const Task task = deal<false, true>(t, b, group, min_columns, INT32_MAX, each, max_shares, kPromptTargetGroups,
+                                        kPromptMinShare, kPromptMinShare, flags);
+    if (task.entry < 0) return;
+    const KvUnit unit = task.unit;
+    const int item = task.entry * each + rest;  // used by shared tiles only
     // the workgroups whose first pair is in this unit
     const int first_block = unit.row_pos / kKvBlock, last_block = (unit.row_pos + unit.row_n - 1) / kKvBlock;
     const int nth = unit.pos / kKvBlock - first_block;
@@ -637,10 +695,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     const int full = min(len / kKvBlock, top + 1);                        // full blocks among 0 .. top
 
     // this workgroup's share of the full blocks; the last share also takes the unfinished block
-    const int shares = max(1, min(splits, full / kPromptMinBlocks));
-    if (split >= shares) return;
-    const int each = (full + shares - 1) / shares;
-    const int from = min(split * each, full), to = min(from + each, full);
+    const int split = task.split, shares = task.shares;
+    const int part_blocks = (full + shares - 1) / shares;
+    const int from = min(split * part_blocks, full), to = min(from + part_blocks, full);
 
     v8h qhi[KK], qlo[KK];
     float col_scale;
@@ -850,7 +907,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nt][r] *= unit_out;
     if (shares > 1) {
-        float *part = partials + (size_t)item * splits * prompt_partial_floats<HD>();
+        float *part = partials + ((size_t)task.place * each + (size_t)rest * shares) * prompt_partial_floats<HD>();
         float *mine = part + (size_t)split * prompt_partial_floats<HD>() + wave * 64 * (HD / 2 + 2) + lane;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -916,17 +973,14 @@ int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const 
                     const AttentionShape &shape, float *d_out) {
     const uint64_t items = (uint64_t)(PER_TOKEN ? (unsigned)b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
     const uint64_t tiles = (shape.columns + 8 * NT - 1) / (8 * NT);
-    // The most workgroups that may share an item, as far as tickets and partial results have room; how
-    // many do is decided on the device, where at most kTargetGroups shares and one rounded up for each item
-    // come out.
+    // The most workgroups that may share an item, as far as there are tickets; how many do is decided on the device.
     const uint64_t slots = items * tiles;
     const uint64_t most = ((uint64_t)t.max_blocks + kMinShare - 1) / kMinShare;
-    const uint64_t room = (uint64_t)RBN_SPLITK_TILES * 1024 / (slots * partial_floats<HD, NT>());
-    uint64_t shares = most < kMaxShares ? most : kMaxShares;
-    shares = shares < room ? shares : room;
-    if (shares < 1 || slots > kMostItems) shares = 1;
+    const uint64_t shares = slots > kMostItems ? 1 : most < kMaxShares ? most : kMaxShares;
+    static_assert(2ull * kTargetGroups * partial_floats<HD, NT>() <= RBN_SPLITK_TILES * 1024ull,
+                  "the partial results of all shares must fit the workspace");
     uint64_t groups = slots * shares;
-    if (shares > 1 && groups > slots + kTargetGroups) groups = slots + kTargetGroups;
+    if (groups > slots + kTargetGroups) groups = slots + kTargetGroups;
     RBN_REQUIRE(groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
     attention_token_kernel<FMT, HD, NT, PER_TOKEN><<<dim3((unsigned)groups), dim3(kTokenThreads), 0, ctx->stream>>>(
         d_q, t, b, l, shape.heads, (int)tiles, (int)shares, shape.max_columns, (float *)ctx->splitk_partials,
@@ -956,15 +1010,16 @@ int launch_prompt_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const
                      const AttentionShape &shape, float *d_out) {
     const uint64_t group = shape.heads / l.kv_heads;
     const uint64_t items = (uint64_t)kv_max_units(b.max_tokens, t.rows) * l.kv_heads * ((group + 3) / 4);
-    // Too few tiles to fill the chip: several workgroups share a tile's keys.
-    uint64_t splits = kPromptTargetGroups / items;
-    const uint64_t room = (uint64_t)RBN_SPLITK_TILES * 1024 / (items * prompt_partial_floats<HD>());
-    splits = splits < room ? splits : room;
-    if (splits < 1 || items > RBN_ATTENTION_ITEMS) splits = 1;
-    RBN_REQUIRE(items * splits < (1ull << 31), "too many tokens in rbn_attention_q8kv");
-    attention_prompt_kernel<FMT, HD><<<dim3((unsigned)(items * splits)), dim3(kPromptThreads), 0, ctx->stream>>>(
-        d_q, t, b, l, shape.heads, (int)splits, shape.max_columns + 1, (float *)ctx->splitk_partials, ctx->attention_tickets, d_out,
-        ctx->dev_flags);
+    // as in launch_token_as
+    const uint64_t shares = items > RBN_ATTENTION_ITEMS ? 1 : kPromptMaxShares;
+    static_assert(2ull * kPromptTargetGroups * prompt_partial_floats<HD>() <= RBN_SPLITK_TILES * 1024ull,
+                  "the partial results of all shares must fit the workspace");
+    uint64_t groups = items * shares;
+    if (groups > items + kPromptTargetGroups) groups = items + kPromptTargetGroups;
+    RBN_REQUIRE(groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
+    attention_prompt_kernel<FMT, HD><<<dim3((unsigned)groups), dim3(kPromptThreads), 0, ctx->stream>>>(
+        d_q, t, b, l, shape.heads, (int)shares, shape.max_columns + 1, (float *)ctx->splitk_partials,
+        ctx->attention_tickets, d_out, ctx->dev_flags);
     RBN_HIP(hipGetLastError());
     return RBN_OK;
 }

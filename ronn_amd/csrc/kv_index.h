@@ -57,28 +57,38 @@ struct KvUnit {
     int row_n;       // tokens of the row in the call
 };
 
-// *bad is set if what the batch says of the unit does not fit the table and the batch's own sizes.
+// The unit whose first token is `i`, from what the batch says of that token (row, pos) and of its row (its first
+// token and the first of the next row); .n = 0 if that does not fit the table and the batch's own sizes.
+KV_FN KvUnit kv_make_unit(const KvTableArgs &t, int tokens, int i, int row, int pos, int row_first, int row_end) {
+    KvUnit r;
+    const int cap = t.max_blocks * kKvBlock;
+    r.n = 0;
+    r.first = i;
+    r.row = row;
+    r.pos = pos;
+    r.row_first = row_first;
+    if (i < 0 || i >= tokens || row < 0 || row >= t.rows || pos < 0 || pos >= cap) return r;
+    if (row_first < 0 || row_first > i || row_end <= i || row_end > tokens) return r;
+    r.row_n = row_end - row_first;
+    r.row_pos = pos - (i - row_first);
+    if (r.row_pos < 0 || r.row_pos + r.row_n > cap) return r;
+    const int left = kKvBlock - (pos & (kKvBlock - 1));
+    r.n = row_end - i < left ? row_end - i : left;
+    return r;
+}
+
+// Unit u of a batch; *bad is set if there is one but what the batch says of it is not sound.
 KV_FN KvUnit kv_resolve_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, bool *bad) {
+    const int tokens = b.count[0] < b.max_tokens ? b.count[0] : b.max_tokens;
     KvUnit r;
     r.n = 0;
-    const int tokens = b.count[0] < b.max_tokens ? b.count[0] : b.max_tokens;
     if (u >= (b.count[1] < b.max_tokens ? b.count[1] : b.max_tokens)) return r;
-    *bad = true;
-    const int i = b.unit[u], cap = t.max_blocks * kKvBlock;
-    if (i < 0 || i >= tokens) return r;
-    r.first = i;
-    r.row = b.row[i];
-    r.pos = b.pos[i];
-    if (r.row < 0 || r.row >= t.rows || r.pos < 0 || r.pos >= cap) return r;
-    r.row_first = b.start[r.row];
-    const int end = b.start[r.row + 1];
-    if (r.row_first < 0 || r.row_first > i || end <= i || end > tokens) return r;
-    r.row_n = end - r.row_first;
-    r.row_pos = r.pos - (i - r.row_first);
-    if (r.row_pos < 0 || r.row_pos + r.row_n > cap) return r;
-    const int left = kKvBlock - (r.pos & (kKvBlock - 1));
-    r.n = end - i < left ? end - i : left;
-    *bad = false;
+    const int i = b.unit[u];
+    const bool token = i >= 0 && i < tokens;
+    const int row = token ? b.row[i] : -1, pos = token ? b.pos[i] : -1;
+    const bool known = row >= 0 && row < t.rows;
+    r = kv_make_unit(t, tokens, i, row, pos, known ? b.start[row] : -1, known ? b.start[row + 1] : -1);
+    *bad = r.n == 0;
     return r;
 }
 
