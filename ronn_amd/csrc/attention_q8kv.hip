@@ -102,16 +102,17 @@ struct Task {
 // workgroups between the busy ones.  Rows with fewer columns than min_columns or more than max_columns get no
 // turn.  `each`: workgroups with the same share of an entry; `target`: shares times `each` wanted in all (one more
 // for each entry can come out, and no more than 2 target belong to entries that are shared); least, most: blocks of
-// a share at least, while that gives no more than a workgroup per CU and beyond.  REVERSE: last entries first.
+// a share at least, while that gives no more than a workgroup per CU and beyond.
 constexpr int kComputeUnits = 256;
 constexpr int kLook = 4;  // rounds of 64 entries looked at together
 
-template <bool PER_TOKEN, bool REVERSE>
+template <bool PER_TOKEN>
 __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b, int group, int min_columns, int max_columns,
                                      int each, int max_shares, int target, int least, int most, unsigned *flags) {
     const int lane = threadIdx.x & 63;
     const int tokens = min(b.count[0], b.max_tokens), count = PER_TOKEN ? tokens : min(b.count[1], b.max_tokens);
-    const int limit = PER_TOKEN ? b.max_tokens : count;  // (tokens are read up to the capacity: no wait for the count)
+    // (read up to what there can be: no wait for the count)
+    const int limit = PER_TOKEN ? b.max_tokens : kv_max_units(b.max_tokens, t.rows);
     Task r;
     r.entry = -1;
     KvUnit mine[kLook];
@@ -121,11 +122,11 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
 #pragma unroll
         for (int k = 0; k < kLook; ++k) {
             const int i = base + 64 * k + lane;
-            at[k] = i >= limit ? -1 : PER_TOKEN ? i : b.unit[REVERSE ? count - 1 - i : i];
+            at[k] = i >= limit ? -1 : PER_TOKEN ? i : b.unit[i];
         }
 #pragma unroll
         for (int k = 0; k < kLook; ++k) {
-            const bool in = at[k] >= 0 && at[k] < b.max_tokens;
+            const bool in = at[k] >= 0 && at[k] < b.max_tokens;  // (behind the count anything may stand there)
             row[k] = in ? b.row[at[k]] : -1;
             pos[k] = in ? b.pos[at[k]] : -1;
         }
@@ -179,7 +180,7 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
             if (r.entry < 0 && behind) {
                 const int owner = (int)__builtin_ctzll(behind), i = base + 64 * k + owner;
                 auto of = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
-                r.entry = REVERSE ? count - 1 - i : i;
+                r.entry = i;
                 r.shares = of(parts);
                 r.split = turn - (of(upto) - r.shares);
                 r.place += of(shared_upto) - (r.shares > 1 ? r.shares : 0);
@@ -253,12 +254,13 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
     __shared__ float s_m[kTokenWaves][8 * NT], s_l[kTokenWaves][8 * NT];
     __shared__ float s_weight[8 * NT][kMaxShares], s_den[8 * NT];
     __shared__ int s_last;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane: branches on it are scalar
     const int c16 = lane & 15, c8 = lane & 7, g = lane >> 4;
     const int group = heads / l.kv_heads;
     // this workgroup's task: an item (token or unit, K/V head, tile of columns) and a share of its blocks
     const int each = l.kv_heads * tiles, rest = blockIdx.x % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
-    const Task task = deal<PER_TOKEN, false>(t, b, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
+    const Task task = deal<PER_TOKEN>(t, b, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
                                              2 * kMinShare, flags);
     if (task.entry < 0) return;
     const int row = task.unit.row, pos = task.unit.pos, first = task.unit.first, n = task.unit.n;
@@ -635,14 +637,14 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
 //  * The (block, head) pairs of a row and a K/V head are numbered block by block; the four waves of a
 //    workgroup take four in a row and share the keys and values, which the workgroup converts
 //    once to f16 in LDS, in operand order: every operand read is one conflict-free 16-byte read per lane.
-//  * The next block's codes are in flight while the present one is used; they are converted into the other LDS
-//    buffer between the scores and the softmax: one barrier per block.
-//  * q and P in f16 as hi + lo, two instructions each (a tile has 32 columns of its own here).  V's scale
-//    goes into P; the output is kept in units of a power of two near the scales so far, with P
-//    shifted up by 2^8, so that neither part of P leaves f16's range: scales within
-//    [2^-4, 4) of the unit use it as it is, others move it (the store's scales span 2^-32 .. 2^9).
+//  * q and P in f16 as hi + lo, two instructions each (a tile has 32 columns of its own here).  V's scale goes
+//    into P; the output is kept in units of a power of two near the scales so far.  Scales within [2^-4, 4)
+//    of the unit use it as it is, others move it (the store's scales span 2^-32 .. 2^9), the running
+//    maximum lags behind by up to 2^8, and P is shifted up by 2^5: its parts reach at most 2^15, and the
+//    smallest step of f16 is 2^-25 or less of the largest weight.
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 constexpr int kPromptThreads = 256;
+constexpr int kShift = 5;                 // log2 of what P is scaled up by
 constexpr int kPromptTargetGroups = 480;  // workgroups that share the tiles' blocks evenly; partial results of twice as many fit
 constexpr int kPromptMinShare = 4;        // blocks a workgroup takes at least before another shares the tile
 constexpr int kPromptMaxShares = 16;
@@ -661,14 +663,14 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     constexpr int NT = HD / 32;   // tiles of dimensions of the output
     constexpr int kTile = kKvBlock * HD;
     constexpr int PER = kTile / kPromptThreads;  // codes of K (and of V) a thread converts: 16 or 8
-    __shared__ __attribute__((aligned(16))) _Float16 s_k[2][kTile], s_v[2][kTile];
+    __shared__ __attribute__((aligned(16))) _Float16 s_k[3][kTile], s_v[3][kTile];
     __shared__ int s_last;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane: branches on it are scalar
     const int group = heads / l.kv_heads;
     const int per_unit = (group + 3) / 4;
-    // (the long ones first)
     const int each = l.kv_heads * per_unit, rest = blockIdx.x % each, kvh = rest % l.kv_heads, z = rest / l.kv_heads;
-    const Task task = deal<false, true>(t, b, group, min_columns, INT32_MAX, each, max_shares, kPromptTargetGroups,
+    const Task task = deal<false>(t, b, group, min_columns, INT32_MAX, each, max_shares, kPromptTargetGroups,
                                         kPromptMinShare, kPromptMinShare, flags);
     if (task.entry < 0) return;
     const KvUnit unit = task.unit;
@@ -678,11 +680,6 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     const int nth = unit.pos / kKvBlock - first_block;
     const int pair0 = (((nth * group + 3) >> 2) + z) * 4;
     if (pair0 >= (nth + 1) * group) return;
-    const int len = min(t.len[unit.row], t.max_blocks * kKvBlock);
-    if (unit.row_pos + unit.row_n > len) {
-        if (tid == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
-        return;
-    }
     const int pairs = (last_block - first_block + 1) * group;
     const int pair = pair0 + wave;
     const bool idle = pair >= pairs;
@@ -692,38 +689,105 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     const int query = own * kKvBlock + col;                               // this lane's position
     const bool real = !idle && query >= unit.row_pos && query < unit.row_pos + unit.row_n;
     const int token = unit.row_first + min(max(query - unit.row_pos, 0), unit.row_n - 1);
-    const int full = min(len / kKvBlock, top + 1);                        // full blocks among 0 .. top
 
-    // this workgroup's share of the full blocks; the last share also takes the unfinished block
-    const int split = task.split, shares = task.shares;
-    const int part_blocks = (full + shares - 1) / shares;
-    const int from = min(split * part_blocks, full), to = min(from + part_blocks, full);
-
-    v8h qhi[KK], qlo[KK];
-    float col_scale;
+    // q and the row's length together; then the pages of the share's first blocks, then their codes, and q is
+    // made ready while those travel
+    float x[KK][8];
     {
         const float *src = q + ((size_t)token * heads + head) * HD + 8 * g;
-        float x[KK][8], m = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             const float4 a = *reinterpret_cast<const float4 *>(src + 16 * kk);
             const float4 c = *reinterpret_cast<const float4 *>(src + 16 * kk + 4);
             x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = a.z, x[kk][3] = a.w;
             x[kk][4] = c.x, x[kk][5] = c.y, x[kk][6] = c.z, x[kk][7] = c.w;
+        }
+    }
+    const int len = __builtin_amdgcn_readfirstlane(min(t.len[unit.row], t.max_blocks * kKvBlock));
+    if (unit.row_pos + unit.row_n > len) {
+        if (tid == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+        return;
+    }
+    const int full = min(len / kKvBlock, top + 1);                        // full blocks among 0 .. top
+
+    // this workgroup's share of the full blocks; the last share also takes the unfinished block
+    const int split = task.split, shares = task.shares;
+    const int part_blocks = (full + shares - 1) / shares;
+    const int from = min(split * part_blocks, full), to = min(from + part_blocks, full), last = to - 1;
+
+    typedef typename CodeVec<PER>::type vcode;  // a thread's codes of one page head
+    struct Codes {
+        vcode k, v;
+    };
+    auto load = [&](Codes &c, int page) __attribute__((always_inline)) {  // (an invalid page loads page 0 and is skipped)
+        const size_t at = ((size_t)max(page, 0) * l.kv_heads + kvh) * kTile;
+        c.k = *reinterpret_cast<const vcode *>(l.k + at + tid * PER);
+        c.v = *reinterpret_cast<const vcode *>(l.v + at + tid * PER);
+    };
+    // What is known of a block: page (-1: skipped), scales, and of V's scale the exponent, logarithm and reciprocal.
+    struct Block {
+        int page, ve;
+        float ks, vs, vlog, vinv;
+    };
+    int pages = -1;  // of 64 blocks, one per lane
+    float kss = 0.0f, vss = 0.0f, vlogs = 0.0f, vinvs = 0.0f;
+    auto fetch = [&](int kb, Codes &c) __attribute__((always_inline)) {  // puts block kb's codes on their way
+        const int at = (kb - from) & 63;
+        if (at == 0) {
+            pages = -1;
+            kss = vss = 0.0f;
+            if (kb + lane < to) {
+                pages = kv_page(t, unit.row, kb + lane);
+                const size_t ph = (size_t)max(pages, 0) * l.kv_heads + kvh;
+                kss = l.k_scale[ph];
+                vss = l.v_scale[ph];
+                if (pages < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+            }
+            vlogs = vss > 0.0f ? __builtin_amdgcn_logf(vss) : 0.0f;
+            vinvs = vss > 0.0f ? 1.0f / vss : 1.0f;
+            // waited for here, once in 64 blocks, and not with every block's codes
+            asm volatile("" : "+v"(pages), "+v"(kss), "+v"(vss));
+        }
+        auto of = [&](float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), at)); };
+        Block x;
+        x.page = __builtin_amdgcn_readlane(pages, at);
+        x.ks = of(kss);
+        x.vs = of(vss);
+        x.ve = exponent_of(x.vs);
+        x.vlog = of(vlogs);
+        x.vinv = of(vinvs);
+        load(c, x.page);
+        return x;
+    };
+    Codes even, odd;
+    Block x0{-1, 0, 0.0f, 0.0f, 0.0f, 1.0f}, x1 = x0;
+    if (from < to) {
+        x0 = fetch(from, even);
+        x1 = fetch(min(from + 1, last), odd);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    v8h qhi[KK], qlo[KK];
+    float col_scale;
+    {
+        float m = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[kk][e]));
-        }
         m = fmaxf(m, __shfl_xor(m, 32));
         const int ex = exponent_of(m);
+        const float down = ldexpf(1.0f, -ex);
         col_scale = ldexpf(HD == 128 ? kLog2eBySqrt128 : kLog2eBySqrt64, ex);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = ldexpf(x[kk][e], -ex);
-                const _Float16 hi = (_Float16)v;
-                qhi[kk][e] = hi;
-                qlo[kk][e] = (_Float16)(v - (float)hi);
+            for (int e = 0; e < 8; e += 2) {
+                const float v0 = x[kk][e] * down, v1 = x[kk][e + 1] * down;
+                const v2h hi = __builtin_convertvector((v2f){v0, v1}, v2h);
+                const v2h lo = __builtin_convertvector(((v2f){v0 - (float)hi[0], v1 - (float)hi[1]}), v2h);
+                qhi[kk][e] = hi[0], qhi[kk][e + 1] = hi[1];
+                qlo[kk][e] = lo[0], qlo[kk][e + 1] = lo[1];
             }
     }
 
@@ -736,7 +800,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         for (int r = 0; r < 16; ++r) o[nt][r] = 0.0f;
 
     // scores of the 32 keys in buffer `buf`: register r is key 8 (r/4) + 4 g + r%4
-    auto scores = [&](int buf) {
+    auto scores = [&](int buf) __attribute__((always_inline)) {
         v16f s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
@@ -748,37 +812,36 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         }
         return s;
     };
-    // softmax and P.V of block kb
-    auto attend = [&](v16f s, int buf, float kscale, float vscale, int kb) {
-        // the unit of the output follows V's scale
-        const int ve = exponent_of(vscale);
-        if (vscale > 0.0f && (ve < vexp - 4 || ve > vexp + 1)) {
+    auto max_of = [&](const v16f &s) __attribute__((always_inline)) {
+        float m = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+        return m;
+    };
+    // What the softmax of a block needs besides its raw scores s and their maximum m (before the masks of a
+    // diagonal block): masks, a running maximum that is near enough, the output's unit.
+    // f: raw score times this is an exponent of two (at least the smallest normal, so that a masked -inf stays
+    // one where the scale is 0); bias: minus the maximum plus log2 of P's shift; inverse: of that shift.
+    float f, bias, inverse;
+    auto settle = [&](v16f &s, float m, const Block &x, bool diagonal) __attribute__((always_inline)) {
+        if (x.vs > 0.0f && (x.ve < vexp - 4 || x.ve > vexp + 1)) {  // the unit of the output follows V's scale
             if (vexp > -200) {
-                const float by = ldexpf(1.0f, vexp - ve);
+                const float by = ldexpf(1.0f, vexp - x.ve);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[nt][r] *= by;
             }
-            vexp = ve;
+            vexp = x.ve;
         }
-        const float shift = ldexpf(vscale, 8 - vexp);
-        const float f = kscale * col_scale;
-        float m = -INFINITY;
-        if (kb == own) {
+        f = fmaxf(x.ks * col_scale, 1.17549435e-38f);
+        if (diagonal) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = 8 * (r >> 2) + 4 * g + (r & 3) <= col ? s[r] * f : -INFINITY;
-                m = fmaxf(m, s[r]);
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] *= f;
-                m = fmaxf(m, s[r]);
-            }
+            for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + 4 * g + (r & 3) <= col ? s[r] : -INFINITY;
+            m = max_of(s);
         }
-        if (__any(m > run_max + 4.0f)) {
+        m *= f;
+        if (__any(m > run_max + 8.0f)) {
             m = fmaxf(m, __shfl_xor(m, 32));
             const float mx = fmaxf(run_max, m);
             const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
@@ -789,28 +852,69 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[nt][r] *= corr;
         }
-        const float ref = run_max == -INFINITY ? 0.0f : run_max;
-        v8h phi[2], plo[2];
+        // (a block of V's that is all zero: any shift will do)
+        const int shift = x.vs > 0.0f ? kShift - vexp : 0;
+        bias = x.vlog + (float)shift - (run_max == -INFINITY ? 0.0f : run_max);
+        inverse = ldexpf(x.vinv, -shift);
+    };
+    // P of the raw scores r and r + 1 as f16 hi + lo; returns their sum.
+    v8h phi[2], plo[2];
+    auto soften = [&](const v16f &s, int r) __attribute__((always_inline)) {
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(s[r], f, bias)), w1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], f, bias));
+        const v2h hi = __builtin_convertvector((v2f){w0, w1}, v2h);
+        const v2h lo = __builtin_convertvector(((v2f){w0 - (float)hi[0], w1 - (float)hi[1]}), v2h);
+        phi[r >> 3][r & 7] = hi[0];
+        phi[r >> 3][(r & 7) + 1] = hi[1];
+        plo[r >> 3][r & 7] = lo[0];
+        plo[r >> 3][(r & 7) + 1] = lo[1];
+        return w0 + w1;
+    };
+    auto key_operand = [&](int buf, int kk) __attribute__((always_inline)) {
+        return *reinterpret_cast<const v8h *>(&s_k[buf][(kk * 64 + lane) * 8]);
+    };
+    auto value_operand = [&](int buf, int i) __attribute__((always_inline)) {  // dimensions 32 (i/2) .., key slots of step i%2
+        return *reinterpret_cast<const v8h *>(&s_v[buf][(i * 64 + lane) * 8]);
+    };
+    // Softmax and P.V of the block in buffer b0 whose raw scores are s; leaves the raw scores of the block in b1 in s
+    // and their maximum in m;
+    // `piece(i)`, i < 2 PER / 8, is other work for the vector units.  Written in the order it is to run in
+    // (the barriers keep the compiler from gathering the operand reads right before their uses and the vector work
+    // in one place): operands two reads ahead, the softmax between the matrix instructions of the scores,
+    // the pieces between those of P.V.
+    auto attend = [&](v16f &s, float &m, int b0, int b1, auto piece) __attribute__((always_inline)) {
+        v16f z;
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(s[r] - ref), p1 = __builtin_amdgcn_exp2f(s[r + 1] - ref);
-            run_sum += p0 + p1;
-            const float w0 = p0 * shift, w1 = p1 * shift;
-            const v2h hi = __builtin_convertvector((v2f){w0, w1}, v2h);
-            const v2h lo = __builtin_convertvector(((v2f){w0 - (float)hi[0], w1 - (float)hi[1]}), v2h);
-            phi[r >> 3][r & 7] = hi[0];
-            phi[r >> 3][(r & 7) + 1] = hi[1];
-            plo[r >> 3][r & 7] = lo[0];
-            plo[r >> 3][(r & 7) + 1] = lo[1];
+        for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+        v8h a[3];
+        a[0] = key_operand(b1, 0);
+        a[1] = key_operand(b1, 1);
+        float sum = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            a[(kk + 2) % 3] = kk + 2 < KK ? key_operand(b1, kk + 2) : value_operand(b0, kk + 2 - KK);
+            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk % 3], qhi[kk], z, 0, 0, 0);
+            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk % 3], qlo[kk], z, 0, 0, 0);
+#pragma unroll
+            for (int r = kk * 16 / KK; r < (kk + 1) * 16 / KK; r += 2) sum += soften(s, r);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        run_sum = fmaf(sum, inverse, run_sum);  // the shift comes out of the sum as it went into P
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2 * NT; ++i) {
+            if (i + 2 < 2 * NT) a[(KK + i + 2) % 3] = value_operand(b0, i + 2);
+            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[(KK + i) % 3], phi[i % 2], o[i / 2], 0, 0, 0);
+            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[(KK + i) % 3], plo[i % 2], o[i / 2], 0, 0, 0);
+            if (i % 2 == 0) piece(i / 2);
+            // their maximum, with a delay that spares the wait for the last of the scores
+            if (i >= 2 * NT - 2) {
+                const int from = i == 2 * NT - 2 ? 0 : 8;
+                if (from == 0) m = z[0];
 #pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const v8h va = *reinterpret_cast<const v8h *>(&s_v[buf][((nt * 2 + s2) * 64 + lane) * 8]);
-                o[nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, phi[s2], o[nt], 0, 0, 0);
-                o[nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, plo[s2], o[nt], 0, 0, 0);
+                for (int r = from; r < from + 8; ++r) m = fmaxf(m, z[r]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s = z;
     };
 
     // ---- the unfinished block first, if it is this share's: f16, rows behind the end zeroed
@@ -830,91 +934,93 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
                 s_v[0][(((d >> 5) * 2 + (key >> 4)) * 64 + 32 * (quad & 1) + ((d + j) & 31)) * 8 + e] = vx[j];
         }
         __syncthreads();
-        if (own == top) attend(scores(0), 0, 1.0f, 1.0f, top);
+        if (own == top) {
+            v16f s = scores(0);
+            float m;
+            settle(s, 0.0f, Block{0, 0, 1.0f, 1.0f, 0.0f, 1.0f}, true);
+            attend(s, m, 0, 0, [](int) {});
+        }
         __syncthreads();
     }
 
     // ---- the share's full blocks
-    typedef typename CodeVec<PER>::type vcode;  // a thread's codes of one page head
-    vcode kc, vc;
-    auto load = [&](int page) {  // (an invalid page loads page 0 and is skipped)
-        const size_t at = ((size_t)max(page, 0) * l.kv_heads + kvh) * kTile + tid * PER;
-        kc = *reinterpret_cast<const vcode *>(l.k + at);
-        vc = *reinterpret_cast<const vcode *>(l.v + at);
-    };
-    auto convert = [&](int buf) {
-        // code byte offset of this thread and what it is: see kv_k_byte and kv_v_byte
+    // Piece i of the conversion of a thread's codes: keys or values of its i/2-th eight (kv_k_byte, kv_v_byte).
+    constexpr int kPieces = 2 * PER / 8;
+    auto convert_piece = [&](const Codes &c, int buf, int piece) __attribute__((always_inline)) {
+        const int h = piece >> 1, byte = tid * PER + 8 * h, chunk = byte >> 4, hh = (byte >> 3) & 1, i = chunk & 15;
+        if (piece & 1) {
+            const int quad = (chunk >> 4) & 3, p = chunk >> 6;
+            const v8h x = codes_to_f16<FMT>(c.v[2 * h], c.v[2 * h + 1]);  // keys 4 quad .. +3, then 16 + 4 quad ..
 #pragma unroll
-        for (int h = 0; h < PER / 8; ++h) {
-            const int byte = tid * PER + 8 * h;
-            const int chunk = byte >> 4, hh = (byte >> 3) & 1;
-            {
-                const int i = chunk & 15, gg = (chunk >> 4) & 3, aj = chunk >> 6, a = aj / (HD / 64), j = aj % (HD / 64);
-                const int kk = (2 * j + hh) * 2 + (gg >> 1);
-                *reinterpret_cast<v8h *>(&s_k[buf][(kk * 64 + 32 * (gg & 1) + 16 * a + i) * 8]) =
-                    codes_to_f16<FMT>(kc[2 * h], kc[2 * h + 1]);
-            }
-            {
-                const int i = chunk & 15, quad = (chunk >> 4) & 3, p = chunk >> 6;
-                const v8h x = codes_to_f16<FMT>(vc[2 * h], vc[2 * h + 1]);  // keys 4 quad .. +3, then 16 + 4 quad ..
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-                    *reinterpret_cast<v4h *>(&s_v[buf][((p * 2 + a) * 64 + 32 * (quad & 1) + 16 * hh + i) * 8 + 4 * (quad >> 1)]) =
-                        a ? __builtin_shufflevector(x, x, 4, 5, 6, 7) : __builtin_shufflevector(x, x, 0, 1, 2, 3);
-            }
+            for (int a = 0; a < 2; ++a)
+                *reinterpret_cast<v4h *>(&s_v[buf][((p * 2 + a) * 64 + 32 * (quad & 1) + 16 * hh + i) * 8 + 4 * (quad >> 1)]) =
+                    a ? __builtin_shufflevector(x, x, 4, 5, 6, 7) : __builtin_shufflevector(x, x, 0, 1, 2, 3);
+        } else {
+            const int gg = (chunk >> 4) & 3, aj = chunk >> 6, a = aj / (HD / 64), j = aj % (HD / 64);
+            const int kk = (2 * j + hh) * 2 + (gg >> 1);
+            *reinterpret_cast<v8h *>(&s_k[buf][(kk * 64 + 32 * (gg & 1) + 16 * a + i) * 8]) =
+                codes_to_f16<FMT>(c.k[2 * h], c.k[2 * h + 1]);
         }
     };
-    int page = -1;
-    float ks = 0.0f, vs = 0.0f;
-    auto look_up = [&](int base) {  // pages and scales of blocks base .. base + 63, one per lane
-        page = -1;
-        ks = vs = 0.0f;
-        if (base + lane < to) {
-            page = kv_page(t, unit.row, base + lane);
-            const size_t ph = (size_t)max(page, 0) * l.kv_heads + kvh;
-            ks = l.k_scale[ph];
-            vs = l.v_scale[ph];
-            if (page < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
-        }
+    auto convert = [&](const Codes &c, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) convert_piece(c, buf, i);
     };
-    for (int base = from; base < to; base += 64) {
-        look_up(base);
-        const int steps = min(64, to - base);
-        load(__builtin_amdgcn_readlane(page, 0));
-        convert(0);
-        load(__builtin_amdgcn_readlane(page, min(1, steps - 1)));
+    static_assert(kPieces <= NT, "a piece for every second operand of P.V at most");
+    // Pipeline, one barrier per block: while block i's softmax runs on the vector units the matrix units do the
+    // scores of block i + 1, block i + 2 is converted into the third buffer, and blocks i + 3 and i + 4 are
+    // on their way.
+    if (from < to) {
+        convert(even, 0);
+        Block x2 = fetch(min(from + 2, last), even);
+        convert(odd, 1);
+        Block x3 = fetch(min(from + 3, last), odd);
         __syncthreads();
-        for (int i = 0; i < steps; ++i) {
-            const int kb = base + i, buf = i & 1;
-            const bool take = kb <= own && __builtin_amdgcn_readlane(page, i) >= 0;
-            v16f s;
-            if (take) s = scores(buf);
-            if (i + 1 < steps) {
-                convert(buf ^ 1);
-                load(__builtin_amdgcn_readlane(page, min(i + 2, steps - 1)));
+        v16f s = scores(0);
+        float m = max_of(s);
+        int b0 = 0, b1 = 1, b2 = 2;  // buffers of blocks i, i + 1, i + 2
+        auto step = [&](int kb, Codes &c) __attribute__((always_inline)) {
+            if (kb <= own && x0.page >= 0) {
+                settle(s, m, x0, kb == own);
+                // (behind the last block the codes are old ones, and never read)
+                attend(s, m, b0, b1, [&](int i) __attribute__((always_inline)) {
+                    if (i < kPieces) convert_piece(c, b2, i);
+                });
+            } else {
+                if (kb < own) s = scores(b1), m = max_of(s);
+                convert(c, b2);
             }
-            if (take)
-                attend(s, buf, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), i)),
-                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), i)), kb);
+            x0 = x1, x1 = x2, x2 = x3;
+            // (behind the last block its codes once more: without a branch the wait for a block's codes leaves
+            // the next one's on their way)
+            x3 = fetch(min(kb + 4, last), c);
+            const int b = b0;
+            b0 = b1, b1 = b2, b2 = b;
             __syncthreads();
+        };
+        int kb = from;
+        for (; kb < last; kb += 2) {
+            step(kb, even);
+            step(kb + 1, odd);
         }
+        if (kb == last) step(kb, even);
     }
 
     run_sum += __shfl_xor(run_sum, 32);
-    const float unit_out = vexp > -200 ? ldexpf(1.0f, vexp - 8) : 0.0f;
+    const float unit_out = vexp > -200 ? ldexpf(1.0f, vexp - kShift) : 0.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nt][r] *= unit_out;
     if (shares > 1) {
         float *part = partials + ((size_t)task.place * each + (size_t)rest * shares) * prompt_partial_floats<HD>();
-        float *mine = part + (size_t)split * prompt_partial_floats<HD>() + wave * 64 * (HD / 2 + 2) + lane;
+        float *mine = part + (size_t)split * prompt_partial_floats<HD>() + wave * 64 * (HD / 2 + 2);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) store_agent(mine + 64 * (nt * 16 + r), o[nt][r]);
-        store_agent(mine + 64 * (HD / 2), run_max);
-        store_agent(mine + 64 * (HD / 2 + 1), run_sum);
+        for (int i = 0; i < 4 * NT; ++i)
+            store_agent(mine + (i * 64 + lane) * 4,
+                        (v4f){o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]});
+        store_agent(mine + 64 * (HD / 2) + lane, run_max);
+        store_agent(mine + 64 * (HD / 2 + 1) + lane, run_sum);
         // published once the stores have completed (vmcnt(0): this wave's, the barrier: everybody's)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -926,25 +1032,33 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         }
         __syncthreads();
         if (!s_last) return;
-        const float *from_part = part + wave * 64 * (HD / 2 + 2) + lane;
-        float m = -INFINITY;
-        for (int sp = 0; sp < shares; ++sp)
-            m = fmaxf(m, load_agent(from_part + (size_t)sp * prompt_partial_floats<HD>() + 64 * (HD / 2)));
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        const float *other = part + wave * 64 * (HD / 2 + 2);
+        float m = -INFINITY, pm[kPromptMaxShares];
+#pragma unroll
+        for (int sp = 0; sp < kPromptMaxShares; ++sp)
+            pm[sp] = sp < shares ? load_agent(other + (size_t)sp * prompt_partial_floats<HD>() + 64 * (HD / 2) + lane) : -INFINITY;
+#pragma unroll
+        for (int sp = 0; sp < kPromptMaxShares; ++sp) m = fmaxf(m, pm[sp]);
         run_sum = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[nt][r] = 0.0f;
+#pragma unroll 1
         for (int sp = 0; sp < shares; ++sp) {
-            const float *p = from_part + (size_t)sp * prompt_partial_floats<HD>();
-            const float pm = load_agent(p + 64 * (HD / 2)), pl = load_agent(p + 64 * (HD / 2 + 1));
+            const float *p = other + (size_t)sp * prompt_partial_floats<HD>();
+            v4f z[4 * NT];
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) z[i] = *reinterpret_cast<const v4f *>(p + (i * 64 + lane) * 4);
+            const float pmax = p[64 * (HD / 2) + lane], pl = p[64 * (HD / 2 + 1) + lane];
             // a share without keys for this query has sum 0; one with nothing but NaN maximum -inf and a NaN sum
-            const float k = pm == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pm - m);
-            run_sum += k * pl;
+            const float k = pmax == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pmax - m);
+            run_sum = fmaf(k, pl, run_sum);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int i = 0; i < 4 * NT; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[nt][r] += k * load_agent(p + 64 * (nt * 16 + r));
+                for (int r = 0; r < 4; ++r) o[i / 4][i % 4 * 4 + r] = fmaf(k, z[i][r], o[i / 4][i % 4 * 4 + r]);
         }
     }
     if (!real) return;
@@ -971,7 +1085,7 @@ struct AttentionShape {
 template <int FMT, int HD, int NT, bool PER_TOKEN>
 int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
                     const AttentionShape &shape, float *d_out) {
-    const uint64_t items = (uint64_t)(PER_TOKEN ? (unsigned)b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
+    const uint64_t items = (uint64_t)(PER_TOKEN ? b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
     const uint64_t tiles = (shape.columns + 8 * NT - 1) / (8 * NT);
     // The most workgroups that may share an item, as far as there are tickets; how many do is decided on the device.
     const uint64_t slots = items * tiles;

@@ -39,13 +39,6 @@ static inline int kv_check_layer(const rbn_kv_layer *l, KvLayerArgs *out, const 
     return RBN_OK;
 }
 
-// Units a batch can have at most: a unit is a (row, block) pair, so no more than the tokens, and a
-// row's n tokens touch at most n / 32 + 2 blocks.
-static inline unsigned kv_max_units(uint64_t max_tokens, uint64_t rows) {
-    const uint64_t by_rows = max_tokens / RBN_KV_BLOCK + 2 * rows;
-    return (unsigned)(max_tokens < by_rows ? max_tokens : by_rows);
-}
-
 // The value a code stands for, before its scale.
 template <int FMT>
 __device__ __forceinline__ float kv_decode(uint8_t c) {

@@ -92,6 +92,13 @@ KV_FN KvUnit kv_resolve_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, 
     return r;
 }
 
+// Units a batch can have at most: a unit is a (row, block) pair, so no more than the tokens, and a
+// row's n tokens touch at most n / 32 + 2 blocks.
+KV_FN int kv_max_units(int max_tokens, int rows) {
+    const int by_rows = max_tokens / RBN_KV_BLOCK + 2 * rows;
+    return max_tokens < by_rows ? max_tokens : by_rows;
+}
+
 // Page of a row's block (both in range), or -1.
 KV_FN int kv_page(const KvTableArgs &t, int row, int block) {
     const int page = t.table[(size_t)row * t.max_blocks + block];
