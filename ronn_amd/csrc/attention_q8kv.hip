@@ -98,17 +98,18 @@ struct Task {
 
 // Deals the batch out in shares of equal size, so that rows of any mix of lengths fill the chip evenly.  Every
 // wave does it for itself: the blocks of all entries give the size of a share, and a running sum of the shares
-// tells whose turn blockIdx.x is: one trip through the batch's arrays for up to 256 entries, no barrier, no idle
+// tells whose turn workgroup `block` is: one trip through the batch's arrays for up to 256 entries, no barrier, no idle
 // workgroups between the busy ones.  Rows with fewer columns than min_columns or more than max_columns get no
 // turn.  `each`: workgroups with the same share of an entry; `target`: shares times `each` wanted in all (one more
 // for each entry can come out, and no more than 2 target belong to entries that are shared); least, most: blocks of
-// a share at least, while that gives no more than a workgroup per CU and beyond.
+// a share at least, while that gives no more than a workgroup per CU and beyond; weigh: a unit's blocks (0: no turn).
 constexpr int kComputeUnits = 256;
 constexpr int kLook = 4;  // rounds of 64 entries looked at together
 
-template <bool PER_TOKEN>
-__device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b, int group, int min_columns, int max_columns,
-                                     int each, int max_shares, int target, int least, int most, unsigned *flags) {
+template <bool PER_TOKEN, typename Weigh>
+__device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b, int block, int group, int min_columns,
+                                     int max_columns, int each, int max_shares, int target, int least, int most,
+                                     unsigned *flags, Weigh weigh) {
     const int lane = threadIdx.x & 63;
     const int tokens = min(b.count[0], b.max_tokens), count = PER_TOKEN ? tokens : min(b.count[1], b.max_tokens);
     // (read up to what there can be: no wait for the count)
@@ -149,12 +150,21 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
                 mine[k] = kv_make_unit(t, tokens, at[k], row[k], pos[k], s0[k], s1[k]);
                 if (i < count && mine[k].n == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
                 const int64_t columns = mine[k].n > 0 ? (int64_t)mine[k].row_n * group : -1;
-                blocks[k] = columns >= min_columns && columns <= max_columns ? pos[k] / kKvBlock + 1 : 0;
+                blocks[k] = columns >= min_columns && columns <= max_columns ? weigh(mine[k]) : 0;
             }
             if (i >= count) blocks[k] = 0;
         }
     };
-    int turn = blockIdx.x / each, share = INT32_MAX / 2;  // turn counts down to the entry
+    if (!PER_TOKEN && max_columns < INT32_MAX) {
+        // often no row is for this kernel: one look at the rows alone tells
+        bool any = false;
+        for (int i = lane; i < t.rows; i += 64) {
+            const int64_t columns = ((int64_t)b.start[i + 1] - b.start[i]) * group;
+            any |= columns > 0 && columns <= max_columns;
+        }
+        if (!__any(any)) return r;
+    }
+    int turn = block / each, share = INT32_MAX / 2;  // turn counts down to the entry
     if (max_shares > 1 || limit <= 64 * kLook) {
         int64_t all = 0;
         for (int base = 0; base < limit; base += 64 * kLook) {
@@ -170,39 +180,74 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
             share = (int)max(min((int64_t)most, max((int64_t)least, all / kComputeUnits)), (all + target - 1) / target);
     }
     r.place = 0;
-    for (int base = 0; base < limit; base += 64 * kLook) {
-        if (limit > 64 * kLook) look(base);
+    auto pick = [&](int base, int k, int owner) {
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+        r.entry = base + 64 * k + owner;
+        r.unit.row = of(mine[k].row);
+        r.unit.pos = of(mine[k].pos);
+        if (PER_TOKEN) {
+            r.unit.first = r.entry;
+            r.unit.n = 1;
+        } else {
+            r.unit.first = of(mine[k].first);
+            r.unit.n = of(mine[k].n);
+            r.unit.row_first = of(mine[k].row_first);
+            r.unit.row_pos = of(mine[k].row_pos);
+            r.unit.row_n = of(mine[k].row_n);
+        }
+    };
+    // Shared entries first, then the others, the large before the small if they are in registers: what is
+    // dispatched last should be small.
+    const bool shared_first = share < INT32_MAX / 2, sorted = shared_first && limit <= 64 * kLook;
+    for (int kind = shared_first ? 0 : 1; kind < (sorted ? 1 : 2); ++kind)
+        for (int base = 0; base < limit; base += 64 * kLook) {
+            if (limit > 64 * kLook) look(base);
 #pragma unroll
-        for (int k = 0; k < kLook; ++k) {
-            const int parts = min(max_shares, (int)(((int64_t)blocks[k] + share - 1) / share));
-            const int upto = wave_scan_i(parts), shared_upto = wave_scan_i(parts > 1 ? parts : 0);
-            const unsigned long long behind = __ballot(turn < upto);
-            if (r.entry < 0 && behind) {
-                const int owner = (int)__builtin_ctzll(behind), i = base + 64 * k + owner;
-                auto of = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
-                r.entry = i;
-                r.shares = of(parts);
-                r.split = turn - (of(upto) - r.shares);
-                r.place += of(shared_upto) - (r.shares > 1 ? r.shares : 0);
-                r.unit.row = of(mine[k].row);
-                r.unit.pos = of(mine[k].pos);
-                if (PER_TOKEN) {
-                    r.unit.first = r.entry;
-                    r.unit.n = 1;
-                } else {
-                    r.unit.first = of(mine[k].first);
-                    r.unit.n = of(mine[k].n);
-                    r.unit.row_first = of(mine[k].row_first);
-                    r.unit.row_pos = of(mine[k].row_pos);
-                    r.unit.row_n = of(mine[k].row_n);
+            for (int k = 0; k < kLook; ++k) {
+                int parts = min(max_shares, (int)(((int64_t)blocks[k] + share - 1) / share));
+                if ((parts > 1) != (kind == 0)) parts = 0;
+                const int upto = wave_scan_i(parts);
+                const unsigned long long behind = __ballot(turn < upto);
+                if (r.entry < 0 && behind) {
+                    const int owner = (int)__builtin_ctzll(behind);
+                    r.shares = __builtin_amdgcn_readlane(parts, owner);
+                    r.split = turn - (__builtin_amdgcn_readlane(upto, owner) - r.shares);
+                    r.place += __builtin_amdgcn_readlane(upto, owner) - r.shares;  // (counts for shared ones only)
+                    pick(base, k, owner);
+                }
+                if (r.entry < 0) {
+                    turn -= __builtin_amdgcn_readlane(upto, 63);
+                    r.place += __builtin_amdgcn_readlane(upto, 63);
                 }
             }
-            if (r.entry < 0) {
-                turn -= __builtin_amdgcn_readlane(upto, 63);
-                r.place += __builtin_amdgcn_readlane(shared_upto, 63);
-            }
+            if (r.entry >= 0) return r;
         }
-        if (r.entry >= 0) return r;
+    if (!sorted) return r;
+    // the entry of one share each that has `turn` such entries before it in the order of their blocks: its number of
+    // blocks by bisection, then its place among equals
+    auto at_least = [&](int n) {
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) c += __popcll(__ballot(blocks[k] >= n && blocks[k] <= share));
+        return c;
+    };
+    if (turn >= at_least(1)) return r;
+    int lo = 1, hi = share + 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (at_least(mid) > turn) lo = mid; else hi = mid;
+    }
+    turn -= at_least(lo + 1);
+    r.split = 0;
+    r.shares = 1;
+#pragma unroll
+    for (int k = 0; k < kLook; ++k) {
+        const unsigned long long equal = __ballot(blocks[k] == lo);
+        if (r.entry < 0 && turn < __popcll(equal)) {
+            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(equal >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)equal, 0));
+            pick(0, k, (int)__builtin_ctzll(__ballot(blocks[k] == lo && before == turn)));
+        }
+        turn -= __popcll(equal);
     }
     return r;
 }
@@ -230,7 +275,7 @@ constexpr int kMinShare = 8;
 constexpr int kTargetGroups = 1536;   // workgroups that share the batch's blocks evenly
 constexpr int kMaxShares = 64;        // one lane for each when they are joined; more cost more there than they gain
 constexpr int kMostItems = 2048;      // more items fill the chip without sharing
-constexpr int kFewColumns = 16;
+constexpr int kFewColumns = 16;        // rows with no more are taken here even if others have more
 
 // floats of one split's partial result: columns x (out, max, sum)
 template <int HD, int NT>
@@ -239,29 +284,41 @@ constexpr int partial_floats() {
 }
 static_assert(kMostItems <= RBN_ATTENTION_ITEMS, "a ticket for every item that is shared");
 
+template <int HD, int NT>
+struct TokenShared {
+    float o[kTokenWaves][8 * NT][HD];
+    _Float16 open[kKvBlock * (HD + 8)];
+    v8h q[NT][HD / 32][64];
+    float m[kTokenWaves][8 * NT], l[kTokenWaves][8 * NT];
+    float weight[8 * NT][kMaxShares], den[8 * NT];
+    int last;
+};
+
 template <int FMT, int HD, int NT, bool PER_TOKEN>
-__global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_token_kernel(
-    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int tiles, int max_shares,
-    int max_columns, float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+__device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int block, const float *__restrict__ q,
+                                              const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
+                                              int tiles, int max_shares, int max_columns, float *__restrict__ partials,
+                                              unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 32;   // k steps of the scores
     constexpr int DT = HD / 16;   // tiles of dimensions of the output
     constexpr int LD = HD / 32;   // 16-byte loads per lane of 32 keys, K and V each
     constexpr int kPitch = HD + 8;
     constexpr int kTile = kKvBlock * HD;
-    __shared__ __attribute__((aligned(16))) float s_o[kTokenWaves][8 * NT][HD];
-    __shared__ __attribute__((aligned(16))) _Float16 s_open[kKvBlock * kPitch];
-    __shared__ v8h s_q[NT][KK][64];
-    __shared__ float s_m[kTokenWaves][8 * NT], s_l[kTokenWaves][8 * NT];
-    __shared__ float s_weight[8 * NT][kMaxShares], s_den[8 * NT];
-    __shared__ int s_last;
+    auto &s_o = shared.o;
+    auto &s_open = shared.open;
+    auto &s_q = shared.q;
+    auto &s_m = shared.m, &s_l = shared.l;
+    auto &s_weight = shared.weight;
+    auto &s_den = shared.den;
+    int &s_last = shared.last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane: branches on it are scalar
     const int c16 = lane & 15, c8 = lane & 7, g = lane >> 4;
     const int group = heads / l.kv_heads;
     // this workgroup's task: an item (token or unit, K/V head, tile of columns) and a share of its blocks
-    const int each = l.kv_heads * tiles, rest = blockIdx.x % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
-    const Task task = deal<PER_TOKEN>(t, b, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
-                                             2 * kMinShare, flags);
+    const int each = l.kv_heads * tiles, rest = block % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
+    const Task task = deal<PER_TOKEN>(t, b, block, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
+                                      2 * kMinShare, flags, [](const KvUnit &u) { return u.pos / kKvBlock + 1; });
     if (task.entry < 0) return;
     const int row = task.unit.row, pos = task.unit.pos, first = task.unit.first, n = task.unit.n;
     const int split = task.split, shares = task.shares;
@@ -645,7 +702,7 @@ __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_toke
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 constexpr int kPromptThreads = 256;
 constexpr int kShift = 5;                 // log2 of what P is scaled up by
-constexpr int kPromptTargetGroups = 480;  // workgroups that share the tiles' blocks evenly; partial results of twice as many fit
+constexpr int kPromptTargetGroups = 288;  // shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288)
 constexpr int kPromptMinShare = 4;        // blocks a workgroup takes at least before another shares the tile
 constexpr int kPromptMaxShares = 16;
 
@@ -655,23 +712,40 @@ constexpr int prompt_partial_floats() {
     return 4 * 64 * (HD / 2 + 2);
 }
 
+template <int HD>
+struct PromptShared {
+    _Float16 k[3][kKvBlock * HD], v[3][kKvBlock * HD];
+    v4f scale[4][64];
+    int page[4][64], ve[4][64], last;
+};
+
 template <int FMT, int HD>
-__global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
-    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int max_shares, int min_columns,
-    float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+__device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int block, const float *__restrict__ q,
+                                               const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
+                                               int max_shares, int min_columns, float *__restrict__ partials,
+                                               unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 16;   // k steps of the scores
     constexpr int NT = HD / 32;   // tiles of dimensions of the output
     constexpr int kTile = kKvBlock * HD;
     constexpr int PER = kTile / kPromptThreads;  // codes of K (and of V) a thread converts: 16 or 8
-    __shared__ __attribute__((aligned(16))) _Float16 s_k[3][kTile], s_v[3][kTile];
-    __shared__ int s_last;
+    auto &s_k = shared.k, &s_v = shared.v;
+    auto &s_scale = shared.scale;
+    auto &s_page = shared.page, &s_ve = shared.ve;
+    int &s_last = shared.last;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane: branches on it are scalar
     const int group = heads / l.kv_heads;
     const int per_unit = (group + 3) / 4;
-    const int each = l.kv_heads * per_unit, rest = blockIdx.x % each, kvh = rest % l.kv_heads, z = rest / l.kv_heads;
-    const Task task = deal<false>(t, b, group, min_columns, INT32_MAX, each, max_shares, kPromptTargetGroups,
-                                        kPromptMinShare, kPromptMinShare, flags);
+    const int each = l.kv_heads * per_unit, rest = block % each, kvh = rest % l.kv_heads, z = rest / l.kv_heads;
+    // a unit counts for the workgroups whose first pair is in it, with the blocks of the first of them
+    auto weigh = [group](const KvUnit &u) {
+        const int first_block = u.row_pos / kKvBlock, last_block = (u.row_pos + u.row_n - 1) / kKvBlock;
+        const int nth = u.pos / kKvBlock - first_block, pair0 = ((nth * group + 3) >> 2) * 4;
+        if (pair0 >= (nth + 1) * group) return 0;
+        return first_block + min(pair0 + 3, (last_block - first_block + 1) * group - 1) / group + 1;
+    };
+    const Task task = deal<false>(t, b, block, group, min_columns, INT32_MAX, each, max_shares, kPromptTargetGroups,
+                                  kPromptMinShare, kPromptMinShare, flags, weigh);
     if (task.entry < 0) return;
     const KvUnit unit = task.unit;
     const int item = task.entry * each + rest;  // used by shared tiles only
@@ -690,8 +764,15 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     const bool real = !idle && query >= unit.row_pos && query < unit.row_pos + unit.row_n;
     const int token = unit.row_first + min(max(query - unit.row_pos, 0), unit.row_n - 1);
 
-    // q and the row's length together; then the pages of the share's first blocks, then their codes, and q is
+    // this workgroup's share of blocks 0 .. top: `from` .. `to`; the last share also takes the unfinished block
+    const int split = task.split, shares = task.shares;
+    const int part_blocks = (top + shares) / shares;
+    const int from = split * part_blocks;
+
+    // q, the pages of the share's first blocks and the row's length together; then the first codes, and q is
     // made ready while those travel
+    int first_pages = -1;
+    if (lane < part_blocks && from + lane <= top) first_pages = kv_page(t, unit.row, from + lane);
     float x[KK][8];
     {
         const float *src = q + ((size_t)token * heads + head) * HD + 8 * g;
@@ -709,11 +790,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         return;
     }
     const int full = min(len / kKvBlock, top + 1);                        // full blocks among 0 .. top
-
-    // this workgroup's share of the full blocks; the last share also takes the unfinished block
-    const int split = task.split, shares = task.shares;
-    const int part_blocks = (full + shares - 1) / shares;
-    const int from = min(split * part_blocks, full), to = min(from + part_blocks, full), last = to - 1;
+    const int to = min(from + part_blocks, full), last = to - 1;
 
     typedef typename CodeVec<PER>::type vcode;  // a thread's codes of one page head
     struct Codes {
@@ -724,43 +801,49 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         c.k = *reinterpret_cast<const vcode *>(l.k + at + tid * PER);
         c.v = *reinterpret_cast<const vcode *>(l.v + at + tid * PER);
     };
-    // What is known of a block: page (-1: skipped), scales, and of V's scale the exponent, logarithm and reciprocal.
+    // What is known of a block: page (-1: skipped), K's scale, and of V's the exponent (kNone: it is 0), logarithm
+    // and reciprocal.  A wave keeps this of 64 blocks in LDS: in registers, their loads would be waited for
+    // together with the codes that are on their way.
     struct Block {
         int page, ve;
-        float ks, vs, vlog, vinv;
+        float ks, vlog, vinv;
     };
-    int pages = -1;  // of 64 blocks, one per lane
-    float kss = 0.0f, vss = 0.0f, vlogs = 0.0f, vinvs = 0.0f;
+    constexpr int kNone = 1000;
     auto fetch = [&](int kb, Codes &c) __attribute__((always_inline)) {  // puts block kb's codes on their way
         const int at = (kb - from) & 63;
+        float ks = 0.0f, vs = 0.0f;
         if (at == 0) {
-            pages = -1;
-            kss = vss = 0.0f;
+            int page = kb == from ? first_pages : -1;
+            if (kb != from && kb + lane < to) page = kv_page(t, unit.row, kb + lane);
             if (kb + lane < to) {
-                pages = kv_page(t, unit.row, kb + lane);
-                const size_t ph = (size_t)max(pages, 0) * l.kv_heads + kvh;
-                kss = l.k_scale[ph];
-                vss = l.v_scale[ph];
-                if (pages < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+                const size_t ph = (size_t)max(page, 0) * l.kv_heads + kvh;
+                ks = l.k_scale[ph];
+                vs = l.v_scale[ph];
+                if (page < 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
             }
-            vlogs = vss > 0.0f ? __builtin_amdgcn_logf(vss) : 0.0f;
-            vinvs = vss > 0.0f ? 1.0f / vss : 1.0f;
-            // waited for here, once in 64 blocks, and not with every block's codes
-            asm volatile("" : "+v"(pages), "+v"(kss), "+v"(vss));
+            s_page[wave][lane] = page;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        auto of = [&](float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), at)); };
         Block x;
-        x.page = __builtin_amdgcn_readlane(pages, at);
-        x.ks = of(kss);
-        x.vs = of(vss);
-        x.ve = exponent_of(x.vs);
-        x.vlog = of(vlogs);
-        x.vinv = of(vinvs);
+        x.page = __builtin_amdgcn_readfirstlane(s_page[wave][at]);
         load(c, x.page);
+        if (at == 0) {
+            const bool some = vs > 0.0f;
+            s_ve[wave][lane] = some ? exponent_of(vs) : kNone;
+            s_scale[wave][lane] = (v4f){ks, some ? __builtin_amdgcn_logf(vs) : 0.0f, some ? 1.0f / vs : 1.0f, 0.0f};
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        x.ve = __builtin_amdgcn_readfirstlane(s_ve[wave][at]);
+        const v4f z = s_scale[wave][at];
+        x.ks = z[0];
+        x.vlog = z[1];
+        x.vinv = z[2];
         return x;
     };
     Codes even, odd;
-    Block x0{-1, 0, 0.0f, 0.0f, 0.0f, 1.0f}, x1 = x0;
+    Block x0{-1, kNone, 0.0f, 0.0f, 1.0f}, x1 = x0;
     if (from < to) {
         x0 = fetch(from, even);
         x1 = fetch(min(from + 1, last), odd);
@@ -824,7 +907,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
     // one where the scale is 0); bias: minus the maximum plus log2 of P's shift; inverse: of that shift.
     float f, bias, inverse;
     auto settle = [&](v16f &s, float m, const Block &x, bool diagonal) __attribute__((always_inline)) {
-        if (x.vs > 0.0f && (x.ve < vexp - 4 || x.ve > vexp + 1)) {  // the unit of the output follows V's scale
+        if (x.ve != kNone && (x.ve < vexp - 4 || x.ve > vexp + 1)) {  // the unit of the output follows V's scale
             if (vexp > -200) {
                 const float by = ldexpf(1.0f, vexp - x.ve);
 #pragma unroll
@@ -853,7 +936,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
                 for (int r = 0; r < 16; ++r) o[nt][r] *= corr;
         }
         // (a block of V's that is all zero: any shift will do)
-        const int shift = x.vs > 0.0f ? kShift - vexp : 0;
+        const int shift = x.ve != kNone ? kShift - vexp : 0;
         bias = x.vlog + (float)shift - (run_max == -INFINITY ? 0.0f : run_max);
         inverse = ldexpf(x.vinv, -shift);
     };
@@ -937,7 +1020,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
         if (own == top) {
             v16f s = scores(0);
             float m;
-            settle(s, 0.0f, Block{0, 0, 1.0f, 1.0f, 0.0f, 1.0f}, true);
+            settle(s, 0.0f, Block{0, 0, 1.0f, 0.0f, 1.0f}, true);
             attend(s, m, 0, 0, [](int) {});
         }
         __syncthreads();
@@ -1072,78 +1155,97 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_prompt_kernel(
                 make_float4(o[nt][4 * r4] * inv, o[nt][4 * r4 + 1] * inv, o[nt][4 * r4 + 2] * inv, o[nt][4 * r4 + 3] * inv);
 }
 
-// What a launch needs besides the descriptors: the columns (tokens x heads of a K/V head) an item is expected
-// to have at most, and the most a row may have to be taken by the first kernel (all others by the second).
-struct AttentionShape {
-    uint32_t head_dim, format;
-    int heads;
-    bool per_token;
-    uint64_t columns;
-    int max_columns;
+// One token per row.
+template <int FMT, int HD, int NT>
+__global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_token_kernel(
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int tiles, int max_shares,
+    float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+    __shared__ __attribute__((aligned(16))) TokenShared<HD, NT> shared;
+    attend_tokens<FMT, HD, NT, true>(shared, blockIdx.x, q, t, b, l, heads, tiles, max_shares, INT32_MAX, partials, tickets,
+                                     out, flags);
+}
+
+// Any number of tokens per row: the first `prompts` workgroups are for rows with more than kFewColumns columns, the
+// others for the rest; one launch, so that a batch of both kinds runs at the same time and one of a single kind does
+// not wait for a launch that finds nothing to do (4.5 us).
+template <int FMT, int HD>
+__global__ __launch_bounds__(kPromptThreads, 2) void attention_batch_kernel(
+    const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int prompts, int prompt_shares,
+    int token_shares, float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out,
+    unsigned *flags) {
+    constexpr int NT = kFewColumns / 8;
+    constexpr size_t kPromptPartials = 2ull * kPromptTargetGroups * prompt_partial_floats<HD>();
+    static_assert(kPromptPartials + 2ull * kTargetGroups * partial_floats<HD, NT>() <= RBN_SPLITK_TILES * 1024ull,
+                  "the partial results of all shares must fit the workspace");
+    static_assert(kTokenThreads == kPromptThreads, "both kinds of workgroup are of one launch");
+    __shared__ union {
+        TokenShared<HD, NT> tokens;
+        PromptShared<HD> prompts;
+    } shared;
+    if ((int)blockIdx.x < prompts)
+        attend_prompts<FMT, HD>(shared.prompts, blockIdx.x, q, t, b, l, heads, prompt_shares, kFewColumns + 1, partials,
+                                tickets, out, flags);
+    else
+        attend_tokens<FMT, HD, NT, false>(shared.tokens, blockIdx.x - prompts, q, t, b, l, heads, 1, token_shares,
+                                          kFewColumns, partials + kPromptPartials, tickets + RBN_ATTENTION_ITEMS, out, flags);
+}
+
+// The most workgroups that may share an item, as far as there are tickets; how many do is decided on the device,
+// where `target` shares and one more for each of `busy` items come out at most.
+struct Grid {
+    uint64_t shares, groups;
 };
+Grid grid_for(uint64_t items, uint64_t busy, uint64_t most_items, uint64_t most_shares, uint64_t target) {
+    Grid g;
+    g.shares = items > most_items || most_shares < 1 ? 1 : most_shares;
+    g.groups = busy * g.shares;
+    if (g.groups > busy + target) g.groups = busy + target;
+    if (g.shares == 1) g.groups = busy;
+    return g;
+}
 
-template <int FMT, int HD, int NT, bool PER_TOKEN>
-int launch_token_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                    const AttentionShape &shape, float *d_out) {
-    const uint64_t items = (uint64_t)(PER_TOKEN ? b.max_tokens : kv_max_units(b.max_tokens, t.rows)) * l.kv_heads;
-    const uint64_t tiles = (shape.columns + 8 * NT - 1) / (8 * NT);
-    // The most workgroups that may share an item, as far as there are tickets; how many do is decided on the device.
-    const uint64_t slots = items * tiles;
+uint64_t token_shares(const KvTableArgs &t) {
     const uint64_t most = ((uint64_t)t.max_blocks + kMinShare - 1) / kMinShare;
-    const uint64_t shares = slots > kMostItems ? 1 : most < kMaxShares ? most : kMaxShares;
-    static_assert(2ull * kTargetGroups * partial_floats<HD, NT>() <= RBN_SPLITK_TILES * 1024ull,
-                  "the partial results of all shares must fit the workspace");
-    uint64_t groups = slots * shares;
-    if (groups > slots + kTargetGroups) groups = slots + kTargetGroups;
-    RBN_REQUIRE(groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
-    attention_token_kernel<FMT, HD, NT, PER_TOKEN><<<dim3((unsigned)groups), dim3(kTokenThreads), 0, ctx->stream>>>(
-        d_q, t, b, l, shape.heads, (int)tiles, (int)shares, shape.max_columns, (float *)ctx->splitk_partials,
+    return most < kMaxShares ? most : kMaxShares;
+}
+
+template <int FMT, int HD, int NT>
+int launch_tokens(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
+                  float *d_out) {
+    const uint64_t tiles = (heads / l.kv_heads + 8 * NT - 1) / (8 * NT), items = (uint64_t)b.max_tokens * l.kv_heads * tiles;
+    const Grid g = grid_for(items, items, kMostItems, token_shares(t), kTargetGroups);
+    RBN_REQUIRE(g.groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
+    attention_token_kernel<FMT, HD, NT><<<dim3((unsigned)g.groups), dim3(kTokenThreads), 0, ctx->stream>>>(
+        d_q, t, b, l, heads, (int)tiles, (int)g.shares, (float *)ctx->splitk_partials, ctx->attention_tickets, d_out,
+        ctx->dev_flags);
+    RBN_HIP(hipGetLastError());
+    return RBN_OK;
+}
+
+template <int FMT, int HD>
+int launch_batch(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
+                 float *d_out) {
+    const uint64_t units = kv_max_units(b.max_tokens, t.rows), per_unit = (heads / l.kv_heads + 3) / 4;
+    const uint64_t items = units * l.kv_heads * per_unit;
+    const Grid p = grid_for(items, items, RBN_ATTENTION_ITEMS, kPromptMaxShares, kPromptTargetGroups);
+    // (a row with few columns has two units at most)
+    const uint64_t few = units < 2ull * t.rows ? units : 2ull * t.rows;
+    const Grid k = grid_for(units * l.kv_heads, few * l.kv_heads, kMostItems, token_shares(t), kTargetGroups);
+    RBN_REQUIRE(p.groups + k.groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
+    attention_batch_kernel<FMT, HD><<<dim3((unsigned)(p.groups + k.groups)), dim3(kPromptThreads), 0, ctx->stream>>>(
+        d_q, t, b, l, heads, (int)p.groups, (int)p.shares, (int)k.shares, (float *)ctx->splitk_partials,
         ctx->attention_tickets, d_out, ctx->dev_flags);
     RBN_HIP(hipGetLastError());
     return RBN_OK;
 }
 
 template <int FMT, int HD>
-int launch_token_of(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                    const AttentionShape &shape, float *d_out) {
-    auto f = shape.per_token ? (shape.columns <= 8 ? launch_token_as<FMT, HD, 1, true> : launch_token_as<FMT, HD, 2, true>)
-                             : (shape.columns <= 8 ? launch_token_as<FMT, HD, 1, false> : launch_token_as<FMT, HD, 2, false>);
-    return f(ctx, d_q, t, b, l, shape, d_out);
-}
-
-int launch_token(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                 const AttentionShape &shape, float *d_out) {
-    auto f = shape.format == RBN_KV_I8
-                 ? (shape.head_dim == 128 ? launch_token_of<RBN_KV_I8, 128> : launch_token_of<RBN_KV_I8, 64>)
-                 : (shape.head_dim == 128 ? launch_token_of<RBN_KV_E4M3, 128> : launch_token_of<RBN_KV_E4M3, 64>);
-    return f(ctx, d_q, t, b, l, shape, d_out);
-}
-
-template <int FMT, int HD>
-int launch_prompt_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                     const AttentionShape &shape, float *d_out) {
-    const uint64_t group = shape.heads / l.kv_heads;
-    const uint64_t items = (uint64_t)kv_max_units(b.max_tokens, t.rows) * l.kv_heads * ((group + 3) / 4);
-    // as in launch_token_as
-    const uint64_t shares = items > RBN_ATTENTION_ITEMS ? 1 : kPromptMaxShares;
-    static_assert(2ull * kPromptTargetGroups * prompt_partial_floats<HD>() <= RBN_SPLITK_TILES * 1024ull,
-                  "the partial results of all shares must fit the workspace");
-    uint64_t groups = items * shares;
-    if (groups > items + kPromptTargetGroups) groups = items + kPromptTargetGroups;
-    RBN_REQUIRE(groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
-    attention_prompt_kernel<FMT, HD><<<dim3((unsigned)groups), dim3(kPromptThreads), 0, ctx->stream>>>(
-        d_q, t, b, l, shape.heads, (int)shares, shape.max_columns + 1, (float *)ctx->splitk_partials,
-        ctx->attention_tickets, d_out, ctx->dev_flags);
-    RBN_HIP(hipGetLastError());
-    return RBN_OK;
-}
-
-int launch_prompt(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l,
-                  const AttentionShape &shape, float *d_out) {
-    auto f = shape.format == RBN_KV_I8
-                 ? (shape.head_dim == 128 ? launch_prompt_as<RBN_KV_I8, 128> : launch_prompt_as<RBN_KV_I8, 64>)
-                 : (shape.head_dim == 128 ? launch_prompt_as<RBN_KV_E4M3, 128> : launch_prompt_as<RBN_KV_E4M3, 64>);
-    return f(ctx, d_q, t, b, l, shape, d_out);
+int launch_as(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
+              uint64_t max_new, float *d_out) {
+    // One token per row: token by token (if a row has more after all, so are they).  Otherwise by the rows' columns.
+    if (max_new > 1) return launch_batch<FMT, HD>(ctx, d_q, t, b, l, heads, d_out);
+    return heads / l.kv_heads <= 8 ? launch_tokens<FMT, HD, 1>(ctx, d_q, t, b, l, heads, d_out)
+                                   : launch_tokens<FMT, HD, 2>(ctx, d_q, t, b, l, heads, d_out);
 }
 
 }  // namespace
@@ -1166,14 +1268,9 @@ int rbn_attention_q8kv(rbn_ctx *ctx, const float *d_q, const rbn_kv_table *table
                 layer->kv_heads);
     RBN_REQUIRE(max_new > 0, "max_new of rbn_attention_q8kv is 0");
     RBN_ENTER(ctx);
-    // One token per row: the first kernel, token by token (if a row has more after all, so are they).  Otherwise
-    // rows with few columns go to the first kernel, the others to the second.
-    const uint64_t group = heads / layer->kv_heads;
-    AttentionShape shape{layer->head_dim, layer->format, (int)heads, max_new == 1, max_new == 1 ? group : kFewColumns,
-                         max_new == 1 ? INT32_MAX : kFewColumns};
-    RBN_CHECK(launch_token(ctx, d_q, t, b, l, shape, d_out));
-    if (max_new > 1) RBN_CHECK(launch_prompt(ctx, d_q, t, b, l, shape, d_out));
-    return RBN_OK;
+    auto launch = layer->format == RBN_KV_I8 ? (layer->head_dim == 128 ? launch_as<RBN_KV_I8, 128> : launch_as<RBN_KV_I8, 64>)
+                                             : (layer->head_dim == 128 ? launch_as<RBN_KV_E4M3, 128> : launch_as<RBN_KV_E4M3, 64>);
+    return launch(ctx, d_q, t, b, l, (int)heads, max_new, d_out);
 }
 
 }  // extern "C"

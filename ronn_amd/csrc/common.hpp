@@ -36,7 +36,7 @@ struct rbn_ctx {
     // context and never moved, so launches captured in a HIP graph stay valid.
     void *splitk_partials = nullptr;
     unsigned *splitk_tickets = nullptr;
-    // tickets of the attention over the paged cache: RBN_ATTENTION_ITEMS (item, column tile) pairs
+    // tickets of the attention over the paged cache: RBN_ATTENTION_ITEMS for each of its two kinds of work
     unsigned *attention_tickets = nullptr;
     // One word of RBN_FLAG_* bits that kernels set when they refuse to do something a host
     // check could not see coming (rbn_device_flags reads and clears it).

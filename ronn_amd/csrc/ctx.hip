@@ -131,8 +131,8 @@ static int create_context(int device, bool adopt, hipStream_t stream, rbn_ctx **
         (e = hipMalloc(&ctx->splitk_partials, (size_t)RBN_SPLITK_TILES * 4096)) != hipSuccess ||
         (e = hipMalloc((void **)&ctx->splitk_tickets, RBN_SPLITK_GROUPS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMemset(ctx->splitk_tickets, 0, RBN_SPLITK_GROUPS * sizeof(unsigned))) != hipSuccess ||
-        (e = hipMalloc((void **)&ctx->attention_tickets, RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
-        (e = hipMemset(ctx->attention_tickets, 0, RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
+        (e = hipMalloc((void **)&ctx->attention_tickets, 2 * RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
+        (e = hipMemset(ctx->attention_tickets, 0, 2 * RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMalloc((void **)&ctx->dev_flags, 256)) != hipSuccess ||
         (e = hipMemset(ctx->dev_flags, 0, 256)) != hipSuccess) {
         int rc = rbn_fail(RBN_ERR_HIP, "context set-up failed: %s", hipGetErrorString(e));
