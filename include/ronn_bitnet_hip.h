@@ -381,8 +381,9 @@ int rbn_token_logprobs_f32(rbn_ctx *ctx, const float *d_logits, uint64_t rows, u
  * therefore does not depend on how its tokens were split into calls:
  *   x = f16(k) of every token (rotated k; v as it is); values beyond f16 are saturated, NaN becomes
  *   0, either raises RBN_FLAG_KV_NONFINITE;
- *   full block: scale = max|x| / 127 (RBN_KV_I8) or / 448 (RBN_KV_E4M3), code = round to nearest even
- *   of x / scale to int8 or e4m3; the cache holds code * scale (0 where the scale is 0).
+ *   full block: scale = max|x| * (1/127) (RBN_KV_I8) or max|x| * (1/448) (RBN_KV_E4M3), the reciprocal
+ *   and the product rounded to f32; code = x / scale, rounded to f32 and then to nearest even to int8 or
+ *   e4m3; the cache holds code * scale (0 where the scale is 0).
  * The descriptors below are HOST structs of device pointers; they are copied into the launches,
  * so they may be reused as soon as a call returns and every call can be captured in a graph
  * (the numbers of rows and tokens may differ from replay to replay: the kernels read them from device
@@ -453,14 +454,16 @@ int rbn_kv_plan(rbn_ctx *ctx, const rbn_kv_table *table, const int32_t *d_new,
 int rbn_rope_kv_store_q8(rbn_ctx *ctx, const float *d_qkv, const rbn_kv_table *table,
                          const rbn_kv_batch *batch, const rbn_kv_layer *layer, uint64_t heads,
                          float theta, float *d_q);
-/* What the cache holds at `count` places (d_row[i], d_pos[i]), by table->d_len: d_k and d_v
- * [count, kv_heads, head_dim] f16, the code times the scale rounded once.  A place outside its
- * row gives zeros and RBN_FLAG_KV_BAD_INDEX. */
+/* What the cache holds at `count` places (d_row[i], d_pos[i]), by table->d_len (after the plan): d_k and d_v
+ * [count, kv_heads, head_dim] f16 (16-byte aligned), the code times the scale rounded once.  A place
+ * outside its row gives zeros and RBN_FLAG_KV_BAD_INDEX. */
 int rbn_kv_read_f16(rbn_ctx *ctx, const rbn_kv_table *table, const rbn_kv_layer *layer,
                     const int32_t *d_row, const int32_t *d_pos, uint64_t count, void *d_k, void *d_v);
 /* Causal attention of a planned and stored batch over the cache: token i of row r attends to positions
  * 0 .. d_pos[i] of r, softmax(q.k / sqrt(head_dim)).v; query head h uses K/V head h / (heads /
- * kv_heads).  d_q is rbn_rope_kv_store_q8's; d_out [max_tokens, heads * head_dim] f32, rows behind the
+ * kv_heads).  table->d_len are the lengths after the plan (of a plan that did not update them in place:
+ * its d_len_out); a row whose tokens end behind its length is left out and raises RBN_FLAG_KV_BAD_INDEX.
+ * d_q is rbn_rope_kv_store_q8's; d_out [max_tokens, heads * head_dim] f32, rows behind the
  * last token left alone; both 16-byte aligned.  max_new is the most tokens that any row has in the call,
  * as far as the host knows (1 for a decode step): it picks the kernels, not the result.  A block
  * whose page is out of range is left out; a token left without any block gets zeros. */

@@ -40,7 +40,7 @@ def to_f16(x):
 def quantise_block(x16, fmt):
     """[32, hd] f16 -> (values the codes stand for, float32 scale), codes as numbers."""
     x = x16.astype(np.float32)
-    scale = np.float32(np.abs(x).max() / np.float32(QMAX[fmt]))
+    scale = np.float32(np.abs(x).max() * np.float32(1 / QMAX[fmt]))
     y = (x / scale).astype(np.float32) if scale > 0 else np.zeros_like(x)
     code = np.round(y) if fmt == "i8" else round_e4m3(y)
     return code.astype(np.float32), scale
