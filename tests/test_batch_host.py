@@ -44,6 +44,7 @@ def test_page_layout_is_a_permutation(host, hd, which):
 
 def units(host, rows, max_blocks, batch, u):
     arr = {k: np.asarray(batch[k], dtype=np.int32) for k in ("start", "row", "pos", "unit", "count")}
+    arr["unit"] = np.concatenate([arr["unit"], np.full(len(arr["row"]) - len(arr["unit"]), -1, np.int32)])
     out = (C.c_int * 7)()
     p = lambda k: arr[k].ctypes.data_as(C.c_void_p)  # noqa: E731
     bad = host.kv_unit_of(rows, max_blocks, len(arr["row"]), p("start"), p("row"), p("pos"), p("unit"), p("count"), u, out)
