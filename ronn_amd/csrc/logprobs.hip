@@ -5,14 +5,13 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kVecs = 8;                             // 16-byte loads of a thread in one sweep
-constexpr int kSweep = kThreads * 4 * kVecs;         // logits of one sweep: 16384
+constexpr int kVecs = 4;                             // 16-byte loads of a thread in one sweep of 8192 logits
 constexpr int kGroups = kThreads / 8;                // groups of eight lanes, for the first threshold
 constexpr int kCandidates = 2048;
 constexpr int kMaxSegments = 16;
-constexpr int kMinSegment = 4096;
+constexpr int kMinSegment = 8192;
 constexpr int kTargetGroups = 512;
-static_assert(kGroups == 64, "one wave ranks the groups' maxima");
+static_assert(kGroups == 64, "a lane per group maximum");
 static_assert(kGroups >= RBN_TOP_MAX, "the top-th largest group maximum bounds the top-th largest logit");
 
 // Orders logits by value, then by the lower index, in one 64-bit number: the value's bits made
@@ -39,14 +38,31 @@ __device__ __forceinline__ float lane_max(float v) {
 struct Stat {
     float m, s, w;
 };
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return Stat{m, a.s + b.s, 0.0f};  // nothing but -inf (s = 0) or NaN (s = NaN)
-    // a part that vanishes against the other (one of nothing but -inf among them) adds nothing, not 0 * -inf;
+template <int CTRL, int ROWMASK, typename F>
+__device__ __forceinline__ float dpp_with(float v, float none, F f) {
+    return f(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWMASK, 0xf, false)));
+}
+// The wave's values brought together by f, in an order that is always the same; `none` leaves a value as it is.
+template <typename F>
+__device__ __forceinline__ float wave_all(float v, float none, F f) {
+    v = dpp_with<0x111, 0xf>(v, none, f);  // row_shr:1
+    v = dpp_with<0x112, 0xf>(v, none, f);  // row_shr:2
+    v = dpp_with<0x114, 0xf>(v, none, f);  // row_shr:4
+    v = dpp_with<0x118, 0xf>(v, none, f);  // row_shr:8
+    v = dpp_with<0x142, 0xa>(v, none, f);  // row_bcast15
+    v = dpp_with<0x143, 0xc>(v, none, f);  // row_bcast31
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// The sets of all lanes as one: each is moved to the common maximum, then the sums are added.
+__device__ __forceinline__ Stat join(Stat a) {
+    const float m = wave_all(a.m, -INFINITY, [](float x, float y) { return fmaxf(x, y); });
+    auto sum = [](float v) { return wave_all(v, 0.0f, [](float x, float y) { return x + y; }); };
+    if (m == -INFINITY) return Stat{m, sum(a.s), 0.0f};  // nothing but -inf (s = 0) or NaN (s = NaN)
+    // a set that vanishes against the others (one of nothing but -inf among them) adds nothing, not 0 * -inf;
     // a NaN in its sum stays
-    const float da = a.m - m, db = b.m - m, ca = expf(da), cb = expf(db);
-    return Stat{m, a.s * ca + b.s * cb,
-                (ca == 0.0f ? 0.0f : ca * (a.w + da * a.s)) + (cb == 0.0f ? 0.0f : cb * (b.w + db * b.s))};
+    const float d = a.m - m, c = expf(d);
+    return Stat{m, sum(a.s * c), sum(c == 0.0f ? 0.0f : c * (a.w + d * a.s))};
 }
 
 // The largest `top` of the n keys in cand, sorted, to out: each key's place is the number of larger ones
@@ -55,22 +71,31 @@ __device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, int top, 
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t key = cand[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) rank += cand[j] > key;
         if (rank < top) out[rank] = key;
     }
 }
 
+typedef float v4f __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ float4 load_once(const float *p) {
+    const v4f x = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p));
+    return {x[0], x[1], x[2], x[3]};
+}
+
 // A row is one segment, or a few that workgroups share if there are few rows; the last workgroup of a row
 // to finish joins them (in the order of the segments).  One pass over the logits:
-//  * 16-byte loads, eight in flight per thread; the exponentials' running maximum per thread.
+//  * 16-byte loads, four in flight per thread; the exponentials' running maximum per thread.
 //  * The top alternatives: the first sweep is held in registers; the top-th largest of the maxima of 64 groups of eight
 //    lanes bounds the top-th largest logit from below, and only logits at or above it (typically no more
 //    than twice `top`) go to a list in LDS, which is ranked by counting.  Later sweeps add what exceeds the
 //    list's last entry (their indices are higher, so equals lose).
 //  * Where the list overflows (many equal logits at the bound) or comes out short (NaN), the segment's
 //    alternatives are found one by one instead, each a pass over the segment.
-// Bound by the reading of the logits; with few rows by latency.
-__global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__restrict__ logits, int vocab, size_t pitch,
+// Bound by the reading of the logits; with few rows by latency.  1000 rows of 100003: 73 us, 5.5 TB/s with four workgroups on a
+// CU (8 waves per SIMD; 93 with the 66 registers of twice the loads in flight, 81 with those loads in 64; 100 with the next
+// sweep's loads ahead of the ranking: its registers spill).  16 rows of 32000: 11 us in segments of 8000, 12 of 4600.
+__global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__restrict__ logits, int vocab, size_t pitch,
                                                                int segments, int seg_len,
                                                                const int32_t *__restrict__ target, int top,
                                                                float *__restrict__ logprob, float *__restrict__ entropy,
@@ -82,8 +107,10 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
     __shared__ Stat s_stat[kWaves];
     __shared__ uint64_t s_best[kWaves];
     __shared__ float s_group[kGroups];
+    __shared__ int s_rank[kGroups];
     __shared__ int s_count, s_last;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane
     const size_t r = blockIdx.x / segments;
     const int seg = blockIdx.x % segments;
     const float *x = logits + r * pitch;
@@ -94,6 +121,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
     const int vecs = (n - head) / 4, tail = n - head - 4 * vecs;
     const int vec_lo = lo + head, tail_lo = vec_lo + 4 * vecs;
     const int sweeps = max(1, (vecs + kThreads * kVecs - 1) / (kThreads * kVecs));
+
+    const int y = logprob && tid == 64 ? target[r] : -1;  // (of use to the row's last workgroup)
+    const float xy = y >= 0 && y < vocab ? x[y] : 0.0f;
 
     Stat st{-INFINITY, 0.0f, 0.0f};
     const int want = min(top, n);
@@ -106,7 +136,7 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
             const int k = v0 + j * kThreads;
-            v[j] = k < vecs ? *reinterpret_cast<const float4 *>(x + vec_lo + 4 * (size_t)k)
+            v[j] = k < vecs ? load_once(x + vec_lo + 4 * (size_t)k)
                             : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         }
         int extra = -1;  // this thread's logit outside the 16-byte part
@@ -142,17 +172,23 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
             gm = lane_max<0x4E>(gm);          // quad_perm [2,3,0,1]
             gm = lane_max<0x141>(gm);         // row_half_mirror: the other four of the eight
             if ((lane & 7) == 0) s_group[tid >> 3] = gm;
+            if (tid < kGroups) s_rank[tid] = 0;
             if (tid == 0) s_count = 0;
             __syncthreads();
-            // every wave ranks the 64 maxima (equals by their place)
-            const float g = s_group[lane];
-            int rank = 0;
-            for (int j = 0; j < kGroups; ++j) {
-                const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j));
-                rank += o > g || (o == g && j < lane);
-            }
-            const unsigned long long at = __ballot(rank == want - 1);
-            bound = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), (int)__builtin_ctzll(at)));
+            // the maxima as unsigned numbers in the same order, the last six bits for their places: all differ.  Each
+            // wave compares them with eight of them.
+            const unsigned u = __float_as_uint(s_group[lane]);
+            const unsigned key = ((u & 0x80000000u ? ~u : u | 0x80000000u) & ~63u) | (unsigned)(63 - lane);
+            int above = 0;
+#pragma unroll
+            for (int j = 0; j < kGroups / kWaves; ++j)
+                above += (unsigned)__builtin_amdgcn_readlane((int)key, wave * (kGroups / kWaves) + j) > key;
+            atomicAdd(&s_rank[lane], above);
+            __syncthreads();
+            const unsigned long long at = __ballot(s_rank[lane] == want - 1);
+            const unsigned low = (unsigned)__builtin_amdgcn_readlane((int)key, (int)__builtin_ctzll(at)) & ~63u;
+            // (below the number of -inf: its last bits were cut off)
+            bound = low < 0x007fffffu ? -INFINITY : __uint_as_float(low & 0x80000000u ? low & 0x7fffffffu : ~low);
         } else {
             if (tid < held) s_cand[tid] = s_top[tid];
             if (tid == 0) s_count = held;
@@ -207,12 +243,11 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
         }
     }
 
-    for (int off = 32; off > 0; off >>= 1)
-        st = join(st, Stat{__shfl_xor(st.m, off), __shfl_xor(st.s, off), __shfl_xor(st.w, off)});
+    const Stat none{-INFINITY, 0.0f, 0.0f};
+    st = join(st);
     if (lane == 0) s_stat[wave] = st;
     __syncthreads();
-    st = s_stat[0];
-    for (int w = 1; w < kWaves; ++w) st = join(st, s_stat[w]);
+    st = join(lane < kWaves ? s_stat[lane] : none);
     int entries = want;
 
     if (segments > 1) {
@@ -243,40 +278,39 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(const float *__re
             s_cand[tid] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(all + p * kPart) + j, __ATOMIC_RELAXED,
                                             __HIP_MEMORY_SCOPE_AGENT);
         }
-        auto stat_of = [&](int p) {
-            const float *f = reinterpret_cast<const float *>(all + p * kPart + RBN_TOP_MAX * 8);
-            return Stat{__hip_atomic_load(f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-                        __hip_atomic_load(f + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-                        __hip_atomic_load(f + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
-        };
-        st = stat_of(0);
-        for (int p = 1; p < segments; ++p) st = join(st, stat_of(p));
+        static_assert(kMaxSegments <= 64, "a lane per partial result");
+        Stat part = none;
+        if (lane < segments) {
+            const float *f = reinterpret_cast<const float *>(all + lane * kPart + RBN_TOP_MAX * 8);
+            part.m = __hip_atomic_load(f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            part.s = __hip_atomic_load(f + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            part.w = __hip_atomic_load(f + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        st = join(part);
         __syncthreads();
         entries = min(top, vocab);
         if (tid < segments * RBN_TOP_MAX && s_cand[tid] != 0) {
             const uint64_t key = s_cand[tid];
             int rank = 0;
-            for (int p = 0; p < segments; ++p)
-                for (int j = 0; j < top; ++j) rank += s_cand[p * RBN_TOP_MAX + j] > key;
+            // (padding is below every key)
+#pragma unroll 16
+            for (int j = 0; j < segments * RBN_TOP_MAX; ++j) rank += s_cand[j] > key;
             if (rank < entries) s_top[rank] = key;
         }
         __syncthreads();
     }
 
     const float log_s = logf(st.s);
-    const bool none = st.m == -INFINITY && st.s == 0.0f;  // nothing but -inf
-    auto lp = [&](float v) { return none ? -INFINITY : (v - st.m) - log_s; };
+    const bool empty = st.m == -INFINITY && st.s == 0.0f;  // nothing but -inf
+    auto lp = [&](float v) { return empty ? -INFINITY : (v - st.m) - log_s; };
     if (tid < top) {
         const bool there = tid < entries;
         const uint64_t key = there ? s_top[tid] : 0;
         top_token[r * top + tid] = there ? key_index(key) : -1;
         top_logprob[r * top + tid] = there ? lp(key_value(key)) : -INFINITY;
     }
-    if (tid == 64 && logprob) {
-        const int y = target[r];
-        logprob[r] = y >= 0 && y < vocab ? lp(x[y]) : 0.0f;
-    }
-    if (tid == 128 && entropy) entropy[r] = none ? 0.0f : log_s - st.w / st.s;
+    if (tid == 64 && logprob) logprob[r] = y >= 0 && y < vocab ? lp(xy) : 0.0f;
+    if (tid == 128 && entropy) entropy[r] = empty ? 0.0f : log_s - st.w / st.s;
 }
 
 }  // namespace
