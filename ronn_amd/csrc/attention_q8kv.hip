@@ -103,7 +103,9 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
     r.entry = -1;
     KvUnit mine[kLook];
     int blocks[kLook];
-    auto look = [&](int base) {
+    // round k of the entries from `base` on has any (the same in all lanes: small batches skip the others' work)
+    auto any_in = [&](int base, int k) { return base + 64 * k < limit; };
+    auto look = [&](int base) __attribute__((always_inline)) {
         int at[kLook], row[kLook], pos[kLook], s0[kLook], s1[kLook];
 #pragma unroll
         for (int k = 0; k < kLook; ++k) {
@@ -126,6 +128,8 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
         }
 #pragma unroll
         for (int k = 0; k < kLook; ++k) {
+            blocks[k] = 0;
+            if (!any_in(base, k)) continue;
             const int i = base + 64 * k + lane;
             if (PER_TOKEN) {
                 mine[k].row = row[k];
@@ -189,7 +193,8 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
             if (limit > 64 * kLook) look(base);
 #pragma unroll
             for (int k = 0; k < kLook; ++k) {
-                int parts = min(max_shares, (int)(((int64_t)blocks[k] + share - 1) / share));
+                if (!any_in(base, k)) continue;
+                int parts = min(max_shares, (int)((unsigned)(blocks[k] + share - 1) / (unsigned)share));
                 if ((parts > 1) != (kind == 0)) parts = 0;
                 const int upto = wave_scan_i(parts);
                 const unsigned long long behind = __ballot(turn < upto);
@@ -213,7 +218,8 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
     auto at_least = [&](int n) {
         int c = 0;
 #pragma unroll
-        for (int k = 0; k < kLook; ++k) c += __popcll(__ballot(blocks[k] >= n && blocks[k] <= share));
+        for (int k = 0; k < kLook; ++k)
+            if (any_in(0, k)) c += __popcll(__ballot(blocks[k] >= n && blocks[k] <= share));
         return c;
     };
     if (turn >= at_least(1)) return r;
@@ -227,6 +233,7 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
     r.shares = 1;
 #pragma unroll
     for (int k = 0; k < kLook; ++k) {
+        if (!any_in(0, k)) continue;
         const unsigned long long equal = __ballot(blocks[k] == lo);
         if (r.entry < 0 && turn < __popcll(equal)) {
             const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(equal >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)equal, 0));
@@ -688,7 +695,9 @@ __device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int b
 constexpr int kPromptThreads = 256;
 constexpr int kShift = 5;                 // log2 of what P is scaled up by
 constexpr int kPromptTargetGroups = 288;  // shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288)
-constexpr int kPromptMinShare = 4;        // blocks a workgroup takes at least before another shares the tile
+// blocks a workgroup takes at least before another shares the tile: partial results cost some 10 us to write, wait for
+// and join, a block 0.75 (one prompt of 512, 20 heads: 27.2 us with 4, 25.5 with 8, 24.7 with 12, 27.9 with 16 or none shared)
+constexpr int kPromptMinShare = 12;
 constexpr int kPromptMaxShares = 16;
 
 // floats of one workgroup's partial result: four waves' registers, maxima and sums, lane by lane
