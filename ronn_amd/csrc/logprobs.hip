@@ -89,9 +89,11 @@ __device__ __forceinline__ float4 load_once(const float *p) {
 //  * The top alternatives: the first sweep is held in registers; the top-th largest of the maxima of 64 groups of eight
 //    lanes bounds the top-th largest logit from below, and only logits at or above it (typically no more
 //    than twice `top`) go to a list in LDS, which is ranked by counting.  Later sweeps add what exceeds the
-//    list's last entry (their indices are higher, so equals lose).
-//  * Where the list overflows (many equal logits at the bound) or comes out short (NaN), the segment's
-//    alternatives are found one by one instead, each a pass over the segment.
+//    list's last entry (their indices are higher, so equals lose).  A sweep with too many of them is looked at once
+//    more, with a bound of its own and no more equals than can count (1000 rows of 100003 with all but 20 logits at one
+//    value: 90 us, before that 2.4 ms by the way below; in ascending order 0.77 ms).
+//  * Where the list overflows even so, or comes out short (NaN), the segment's alternatives are found one by one
+//    instead, each a pass over the segment.
 // Bound by the reading of the logits; with few rows by latency.  1000 rows of 100003: 73 us, 5.5 TB/s with four workgroups on a
 // CU (8 waves per SIMD; 93 with the 66 registers of twice the loads in flight, 81 with those loads in 64; 100 with the next
 // sweep's loads ahead of the ranking: its registers spill).  16 rows of 32000: 11 us in segments of 8000, 12 of 4600.
@@ -108,7 +110,7 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
     __shared__ uint64_t s_best[kWaves];
     __shared__ float s_group[kGroups];
     __shared__ int s_rank[kGroups];
-    __shared__ int s_count, s_last;
+    __shared__ int s_count, s_first, s_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane
     const size_t r = blockIdx.x / segments;
@@ -166,14 +168,15 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
         add(xe);
         if (top == 0 || slow) continue;
 
-        bool first = sweep == 0;
-        if (first) {
+        const bool first = sweep == 0;
+        // The want-th largest of the maxima of 64 groups of eight lanes in this sweep; sets the count to `entries`.
+        auto threshold = [&](int entries) {
             float gm = lane_max<0xB1>(here);  // quad_perm [1,0,3,2]
             gm = lane_max<0x4E>(gm);          // quad_perm [2,3,0,1]
             gm = lane_max<0x141>(gm);         // row_half_mirror: the other four of the eight
             if ((lane & 7) == 0) s_group[tid >> 3] = gm;
             if (tid < kGroups) s_rank[tid] = 0;
-            if (tid == 0) s_count = 0;
+            if (tid == 0) s_count = entries, s_first = INT32_MAX;
             __syncthreads();
             // the maxima as unsigned numbers in the same order, the last six bits for their places: all differ.  Each
             // wave compares them with eight of them.
@@ -185,21 +188,23 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
                 above += (unsigned)__builtin_amdgcn_readlane((int)key, wave * (kGroups / kWaves) + j) > key;
             atomicAdd(&s_rank[lane], above);
             __syncthreads();
-            const unsigned long long at = __ballot(s_rank[lane] == want - 1);
-            const unsigned low = (unsigned)__builtin_amdgcn_readlane((int)key, (int)__builtin_ctzll(at)) & ~63u;
-            // (below the number of -inf: its last bits were cut off)
-            bound = low < 0x007fffffu ? -INFINITY : __uint_as_float(low & 0x80000000u ? low & 0x7fffffffu : ~low);
+            // (equal but for those bits may stand in any order: the least of the first `want` it is)
+            return wave_all(s_rank[lane] < want ? s_group[lane] : INFINITY, INFINITY, [](float x, float y) { return fminf(x, y); });
+        };
+        if (tid < held) s_cand[tid] = s_top[tid];
+        if (first) {
+            bound = threshold(0);
         } else {
-            if (tid < held) s_cand[tid] = s_top[tid];
             if (tid == 0) s_count = held;
             __syncthreads();
         }
+        auto put = [&](float a, int i) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kCandidates) s_cand[at] = order_key(a, (unsigned)i);
+        };
         if (first ? here >= bound : here > bound) {
             auto take = [&](float a, int i) {
-                if (first ? a >= bound : a > bound) {
-                    const int at = atomicAdd(&s_count, 1);
-                    if (at < kCandidates) s_cand[at] = order_key(a, (unsigned)i);
-                }
+                if (first ? a >= bound : a > bound) put(a, i);
             };
 #pragma unroll
             for (int j = 0; j < kVecs; ++j) {
@@ -209,8 +214,32 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
             if (extra >= 0) take(xe, extra);
         }
         __syncthreads();
-        const int found = s_count;
+        int found = s_count;
         const int so_far = min(n, (sweep == sweeps - 1 ? n : head + 4 * kThreads * kVecs * (sweep + 1)));
+        if (found > kCandidates) {
+            // too many at the bound (masked logits, say) or above it (a row in ascending order): the sweep once more, with
+            // the bound that it gives itself, and of equals at the bound those from the first on that can count if
+            // nothing else stands among them
+            __syncthreads();
+            bound = fmaxf(bound, threshold(held));
+            const int from = first ? lo : vec_lo + 4 * kThreads * kVecs * sweep, to = lo + so_far;
+            if (tid < held) s_cand[tid] = s_top[tid];
+#pragma unroll 1
+            for (int i = from + tid; i < to; i += kThreads)
+                if (x[i] == bound) {
+                    atomicMin(&s_first, i);
+                    break;
+                }
+            __syncthreads();
+            const int near = s_first < INT32_MAX - RBN_TOP_MAX ? s_first + want : s_first;
+#pragma unroll 1
+            for (int i = from + tid; i < to; i += kThreads) {
+                const float a = x[i];
+                if (a > bound || (a == bound && i < near)) put(a, i);
+            }
+            __syncthreads();
+            found = s_count;
+        }
         if (found > kCandidates || found < min(want, so_far)) {
             slow = true;
         } else if (first || found > held) {

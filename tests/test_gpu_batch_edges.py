@@ -289,3 +289,19 @@ def test_logprobs_of_negative_and_nearly_equal_logits(ctx):
     mixed = np.where(rng.random(vocab) < 0.999, -np.inf, rng.normal(-50, 1, vocab)).astype(np.float32)
     x = np.stack([near, tiny, low, lonely, mixed, -np.abs(rng.normal(0, 1e30, vocab)).astype(np.float32)])
     check_logprobs(ctx, x, [0, 1, 19999, 17, 5, 6], 32)
+
+
+@pytest.mark.parametrize("mask", [-np.inf, -1e9, -10000.0, float(np.finfo(np.float32).min), 0.0])
+def test_logprobs_of_masked_rows(ctx, mask):
+    """Nearly all logits at one value, as a constrained choice leaves them: the rest by value, then the lowest indices; also with
+    smaller logits at the front, NaN among them, and fewer left than are asked for in one stretch but not in another."""
+    rng = np.random.default_rng(3)
+    for vocab in (9000, 50021):
+        x = np.full((8, vocab), mask, np.float32)
+        for r, n in enumerate((0, 1, 5, 19, 20, 300, 40, 6)):
+            at = rng.choice(vocab, n, replace=False)
+            x[r, at] = rng.normal(5, 2, n)
+        x[6, :50] = -2e9 if np.isfinite(mask) and mask > -1e30 else mask
+        x[7, [3, 4000, 8999]] = np.nan
+        check_logprobs(ctx, x, rng.integers(0, vocab, 8), 20)
+        check_logprobs(ctx, x[:, :vocab - 3], rng.integers(0, vocab - 3, 8), 32, pitch=vocab + 2, shift=1)
