@@ -91,6 +91,54 @@ struct Task {
 constexpr int kComputeUnits = 256;
 constexpr int kLook = 4;  // rounds of 64 entries looked at together
 
+// Where nothing is shared, an entry for each workgroup, found without looking at the others: a token, a unit, or, for
+// rows with few columns, the first or second of a row's at most two blocks.
+template <bool PER_TOKEN, typename Weigh>
+__device__ __forceinline__ Task deal_one(const KvTableArgs &t, const KvBatchArgs &b, int turn, int tokens, int count, int group,
+                                         int min_columns, int max_columns, unsigned *flags, Weigh weigh) {
+    Task r;
+    r.entry = -1;
+    r.split = r.place = 0;
+    r.shares = 1;
+    if (PER_TOKEN) {
+        if (turn >= count) return r;
+        r.entry = r.unit.first = turn;
+        r.unit.n = 1;
+        r.unit.row = b.row[turn];
+        r.unit.pos = b.pos[turn];
+        return r;
+    }
+    int i, row;
+    if (max_columns == INT32_MAX) {
+        if (turn >= count) return r;
+        i = b.unit[turn];
+        row = i >= 0 && i < b.max_tokens ? b.row[i] : -1;
+    } else {
+        row = turn >> 1;
+        if (row >= t.rows) return r;
+        i = b.start[row];
+    }
+    const bool known = row >= 0 && row < t.rows && i >= 0 && i < b.max_tokens;
+    const int first = known ? b.start[row] : -1, end = known ? b.start[row + 1] : -1;
+    int pos = known ? b.pos[i] : -1;
+    if (max_columns < INT32_MAX) {
+        if (end <= first) return r;  // no tokens
+        if (turn & 1) {
+            i += kKvBlock - (pos & (kKvBlock - 1));
+            pos += kKvBlock - (pos & (kKvBlock - 1));
+            if (i >= end) return r;
+        }
+    }
+    r.unit = kv_make_unit(t, tokens, i, row, pos, first, end);
+    if (r.unit.n == 0) {
+        if (threadIdx.x == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
+        return r;
+    }
+    const int64_t columns = (int64_t)r.unit.row_n * group;
+    if (columns >= min_columns && columns <= max_columns && weigh(r.unit) > 0) r.entry = turn;
+    return r;
+}
+
 template <bool PER_TOKEN, typename Weigh>
 __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b, int block, int group, int min_columns,
                                      int max_columns, int each, int max_shares, int target, int least, int most,
@@ -144,30 +192,29 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
             if (i >= count) blocks[k] = 0;
         }
     };
-    if (!PER_TOKEN && max_columns < INT32_MAX) {
-        // often no row is for this kernel: one look at the rows alone tells
+    if (max_shares == 1) return deal_one<PER_TOKEN>(t, b, block / each, tokens, count, group, min_columns, max_columns, flags, weigh);
+    if (!PER_TOKEN && (max_columns < INT32_MAX || limit > 64 * kLook)) {
+        // often no row is for this kind of workgroup: one look at the rows alone tells
         bool any = false;
         for (int i = lane; i < t.rows; i += 64) {
             const int64_t columns = ((int64_t)b.start[i + 1] - b.start[i]) * group;
-            any |= columns > 0 && columns <= max_columns;
+            any |= columns > 0 && columns >= min_columns && columns <= max_columns;
         }
         if (!__any(any)) return r;
     }
-    int turn = block / each, share = INT32_MAX / 2;  // turn counts down to the entry
-    if (max_shares > 1 || limit <= 64 * kLook) {
-        int64_t all = 0;
-        for (int base = 0; base < limit; base += 64 * kLook) {
-            look(base);
-            int sum = 0;
+    int64_t all = 0;
+    int longest = 0;  // of the entries of this lane
+    for (int base = 0; base < limit; base += 64 * kLook) {
+        look(base);
+        int sum = 0;
 #pragma unroll
-            for (int k = 0; k < kLook; ++k) sum += blocks[k];
-            all += wave_sum_i(sum);
-        }
-        if (all == 0) return r;
-        all *= each;
-        if (max_shares > 1)
-            share = (int)max(min((int64_t)most, max((int64_t)least, all / kComputeUnits)), (all + target - 1) / target);
+        for (int k = 0; k < kLook; ++k) sum += blocks[k], longest = max(longest, blocks[k]);
+        all += wave_sum_i(sum);
     }
+    if (all == 0) return r;
+    all *= each;
+    const int share = (int)max(min((int64_t)most, max((int64_t)least, all / kComputeUnits)), (all + target - 1) / target);
+    int turn = block / each;  // counts down to the entry
     r.place = 0;
     auto pick = [&](int base, int k, int owner) {
         auto of = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
@@ -187,8 +234,8 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
     };
     // Shared entries first, then the others, the large before the small if they are in registers: what is
     // dispatched last should be small.
-    const bool shared_first = share < INT32_MAX / 2, sorted = shared_first && limit <= 64 * kLook;
-    for (int kind = shared_first ? 0 : 1; kind < (sorted ? 1 : 2); ++kind)
+    const bool sorted = limit <= 64 * kLook;
+    for (int kind = __any(longest > share) ? 0 : 1; kind < (sorted ? 1 : 2); ++kind)
         for (int base = 0; base < limit; base += 64 * kLook) {
             if (limit > 64 * kLook) look(base);
 #pragma unroll
@@ -1224,7 +1271,8 @@ int launch_batch(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvB
     const Grid p = grid_for(items, items, RBN_ATTENTION_ITEMS, kPromptMaxShares, kPromptTargetGroups);
     // (a row with few columns has two units at most)
     const uint64_t few = units < 2ull * t.rows ? units : 2ull * t.rows;
-    const Grid k = grid_for(units * l.kv_heads, few * l.kv_heads, kMostItems, token_shares(t), kTargetGroups);
+    Grid k = grid_for(units * l.kv_heads, few * l.kv_heads, kMostItems, token_shares(t), kTargetGroups);
+    if (k.shares == 1) k.groups = 2ull * t.rows * l.kv_heads;
     RBN_REQUIRE(p.groups + k.groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
     attention_batch_kernel<FMT, HD><<<dim3((unsigned)(p.groups + k.groups)), dim3(kPromptThreads), 0, ctx->stream>>>(
         d_q, t, b, l, heads, (int)p.groups, (int)p.shares, (int)k.shares, (float *)ctx->splitk_partials,
