@@ -66,20 +66,36 @@ class PagedKVCache:
         b.max_tokens = max_tokens
         return b
 
+    def _held(self, what: str, buf: DeviceBuffer, nbytes: int):
+        if buf.nbytes < nbytes:
+            raise ValueError("%s holds %d bytes, %d are needed" % (what, buf.nbytes, nbytes))
+
+    def _layer(self, layer: int):
+        if not 0 <= layer < self.layers:
+            raise ValueError("layer %d is outside [0, %d)" % (layer, self.layers))
+        return self._layers[layer]
+
     def plan(self, d_new: DeviceBuffer, batch=None):
         """Advances the rows by d_new [rows] int32 (n > 0: n tokens, 0: none, < 0: the row ends)."""
+        self._held("d_new", d_new, 4 * self.rows)
         check(self.lib.rbn_kv_plan(self.ctx.handle, self._table, d_new.ptr, batch or self._batch, self.d_len.ptr,
                                    self.d_ring_state.ptr))
 
     def store(self, layer: int, d_qkv: DeviceBuffer, heads: int, theta: float, d_q: DeviceBuffer, batch=None):
-        """Rotates q into d_q and stores k and v of the planned tokens."""
-        check(self.lib.rbn_rope_kv_store_q8(self.ctx.handle, d_qkv.ptr, self._table, batch or self._batch,
-                                            self._layers[layer], heads, float(theta), d_q.ptr))
+        """Rotates q into d_q and stores k and v of the planned tokens.  d_qkv and d_q have room for as many tokens as
+        the batch may have."""
+        batch, kv = batch or self._batch, self._layer(layer)
+        self._held("d_qkv", d_qkv, 4 * batch.max_tokens * (heads + 2 * self.kv_heads) * self.head_dim)
+        self._held("d_q", d_q, 4 * batch.max_tokens * heads * self.head_dim)
+        check(self.lib.rbn_rope_kv_store_q8(self.ctx.handle, d_qkv.ptr, self._table, batch, kv, heads, float(theta), d_q.ptr))
 
     def attend(self, layer: int, d_q: DeviceBuffer, heads: int, max_new: int, d_out: DeviceBuffer, batch=None):
-        """Causal attention of the planned tokens over their rows."""
-        check(self.lib.rbn_attention_q8kv(self.ctx.handle, d_q.ptr, self._table, batch or self._batch,
-                                          self._layers[layer], heads, max_new, d_out.ptr))
+        """Causal attention of the planned tokens over their rows.  d_q and d_out have room for as many tokens as the
+        batch may have."""
+        batch, kv = batch or self._batch, self._layer(layer)
+        for what, buf in (("d_q", d_q), ("d_out", d_out)):
+            self._held(what, buf, 4 * batch.max_tokens * heads * self.head_dim)
+        check(self.lib.rbn_attention_q8kv(self.ctx.handle, d_q.ptr, self._table, batch, kv, heads, max_new, d_out.ptr))
 
     def read(self, layer: int, rows, positions):
         """What the cache holds at the places (rows[i], positions[i]): K and V [n, kv_heads, head_dim] float16."""
@@ -89,7 +105,7 @@ class PagedKVCache:
         n = rows.size * self.kv_heads * self.head_dim
         d_k, d_v = self.ctx.alloc(2 * n), self.ctx.alloc(2 * n)
         d_rows, d_pos = self.ctx.to_device(rows), self.ctx.to_device(positions)
-        check(self.lib.rbn_kv_read_f16(self.ctx.handle, self._table, self._layers[layer], d_rows.ptr, d_pos.ptr,
+        check(self.lib.rbn_kv_read_f16(self.ctx.handle, self._table, self._layer(layer), d_rows.ptr, d_pos.ptr,
                                        rows.size, d_k.ptr, d_v.ptr))
         shape = (rows.size, self.kv_heads, self.head_dim)
         return d_k.download(np.float16, n).reshape(shape), d_v.download(np.float16, n).reshape(shape)

@@ -199,6 +199,31 @@ def test_attention_leaves_out_rows_behind_their_length(ctx):
     rig.cache.d_len.upload(good)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(200, 1), (1024, 1), (256, 256)])
+def test_attention_of_many_heads(ctx, heads, kv_heads):
+    rig = Rig(ctx, heads, kv_heads, 64, "i8", rows=2, max_len=128, max_tokens=64, seed=heads)
+    q = rig.step([40, 20])
+    rig.check_attention(q, 40, sample=4)
+    q = rig.step([1, 13])
+    for hint in (13, 1):
+        rig.check_attention(q, hint, sample=4)
+    rig.check_cache()
+    assert ctx.device_flags() == 0
+
+
+def test_cache_checks_its_buffers(ctx):
+    rig = Rig(ctx, 4, 2, 64, "i8", rows=2, max_len=128, max_tokens=32)
+    small, qkv = ctx.alloc(4), ctx.alloc(4 * 32 * rig.width)
+    for call in (lambda: rig.cache.plan(small), lambda: rig.cache.store(0, small, 4, 1e4, rig.d_q),
+                 lambda: rig.cache.store(0, qkv, 4, 1e4, small), lambda: rig.cache.store(1, qkv, 4, 1e4, rig.d_q),
+                 lambda: rig.cache.store(-1, qkv, 4, 1e4, rig.d_q), lambda: rig.cache.attend(0, small, 4, 1, rig.d_out),
+                 lambda: rig.cache.attend(0, rig.d_q, 4, 1, small), lambda: rig.cache.attend(2, rig.d_q, 4, 1, rig.d_out),
+                 lambda: rig.cache.attend(0, rig.d_q, 8, 1, rig.d_out), lambda: rig.cache.read(1, [0], [0]),
+                 lambda: rig.cache.batch(33), lambda: rig.cache.batch(0)):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ---- several at once -------------------------------------------------------------------------------
 def test_two_graphs_of_a_context_share_its_workspace(ctx):
     """Two captured steps with shared rows, launched in turn without a wait, against eager calls: the same bits every time."""
