@@ -390,7 +390,7 @@ int rbn_token_logprobs_f32(rbn_ctx *ctx, const float *d_logits, uint64_t rows, u
  * memory).  Numbers out of range in device memory never lead outside the buffers: the item is left
  * out and RBN_FLAG_KV_BAD_INDEX raised.  Which rows, pages and calls belong together is the caller's
  * affair: a page handed out twice, or two rows of d_table sharing a page that one of them
- * still fills, gives wrong values. */
+ * still fills, gives wrong values.  The buffers of a call do not overlap except where it says so. */
 #define RBN_KV_BLOCK 32
 #define RBN_KV_MAX_ROWS 2048
 #define RBN_KV_MAX_BLOCKS (1u << 20)  /* of one row */

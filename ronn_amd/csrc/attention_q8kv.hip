@@ -1255,7 +1255,6 @@ int launch_tokens(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const Kv
                   float *d_out) {
     const uint64_t tiles = (heads / l.kv_heads + 8 * NT - 1) / (8 * NT), items = (uint64_t)b.max_tokens * l.kv_heads * tiles;
     const Grid g = grid_for(items, items, kMostItems, token_shares(t), kTargetGroups);
-    RBN_REQUIRE(g.groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
     attention_token_kernel<FMT, HD, NT><<<dim3((unsigned)g.groups), dim3(kTokenThreads), 0, ctx->stream>>>(
         d_q, t, b, l, heads, (int)tiles, (int)g.shares, (float *)ctx->splitk_partials, ctx->attention_tickets, d_out,
         ctx->dev_flags);
@@ -1273,7 +1272,6 @@ int launch_batch(rbn_ctx *ctx, const float *d_q, const KvTableArgs &t, const KvB
     const uint64_t few = units < 2ull * t.rows ? units : 2ull * t.rows;
     Grid k = grid_for(units * l.kv_heads, few * l.kv_heads, kMostItems, token_shares(t), kTargetGroups);
     if (k.shares == 1) k.groups = 2ull * t.rows * l.kv_heads;
-    RBN_REQUIRE(p.groups + k.groups < (1ull << 31), "too many tokens in rbn_attention_q8kv");
     attention_batch_kernel<FMT, HD><<<dim3((unsigned)(p.groups + k.groups)), dim3(kPromptThreads), 0, ctx->stream>>>(
         d_q, t, b, l, heads, (int)p.groups, (int)p.shares, (int)k.shares, (float *)ctx->splitk_partials,
         ctx->attention_tickets, d_out, ctx->dev_flags);
@@ -1309,6 +1307,14 @@ int rbn_attention_q8kv(rbn_ctx *ctx, const float *d_q, const rbn_kv_table *table
                 "heads (%llu) must be a multiple of kv_heads (%u), at most 1024", (unsigned long long)heads,
                 layer->kv_heads);
     RBN_REQUIRE(max_new > 0, "max_new of rbn_attention_q8kv is 0");
+    // a launch holds fewer than 2^32 threads
+    const uint64_t group = heads / layer->kv_heads, tile = group <= 8 ? 8 : 16;
+    const uint64_t groups =
+        max_new > 1 ? ((uint64_t)kv_max_units(b.max_tokens, t.rows) * ((group + 3) / 4) + 2ull * t.rows) * layer->kv_heads
+                    : (uint64_t)b.max_tokens * ((group + tile - 1) / tile) * layer->kv_heads;
+    RBN_REQUIRE(groups + kTargetGroups + kPromptTargetGroups < (1ull << 24),
+                "too much for one call of rbn_attention_q8kv (max_tokens %llu, kv_heads %u, heads %llu)",
+                (unsigned long long)batch->max_tokens, layer->kv_heads, (unsigned long long)heads);
     RBN_ENTER(ctx);
     auto launch = layer->format == RBN_KV_I8 ? (layer->head_dim == 128 ? launch_as<RBN_KV_I8, 128> : launch_as<RBN_KV_I8, 64>)
                                              : (layer->head_dim == 128 ? launch_as<RBN_KV_E4M3, 128> : launch_as<RBN_KV_E4M3, 64>);

@@ -401,6 +401,7 @@ int rbn_rope_kv_store_q8(rbn_ctx *ctx, const float *d_qkv, const rbn_kv_table *t
     RBN_REQUIRE(theta > 0.0f && theta <= 3.4e38f, "theta must be positive and finite");
     RBN_ENTER(ctx);
     const unsigned groups = (unsigned)kv_max_units(batch->max_tokens, table->rows) * layer->kv_heads;
+    static_assert((RBN_KV_MAX_TOKENS / RBN_KV_BLOCK + 2ull * RBN_KV_MAX_ROWS) * 1024 * 256 < 1ull << 32, "threads of a launch");
     RopeFactors factors;
     factors.turn = 0.63661977236758134308;
     for (int i = 0; i < 6; ++i) factors.bit[i] = exp2(-2.0 * (1 << i) / layer->head_dim * log2((double)theta));
@@ -424,7 +425,7 @@ int rbn_kv_read_f16(rbn_ctx *ctx, const rbn_kv_table *table, const rbn_kv_layer 
     RBN_REQUIRE(count > 0 && count < (1ull << 31), "bad count in rbn_kv_read_f16");
     RBN_REQUIRE(aligned16(d_k) && aligned16(d_v), "d_k and d_v of rbn_kv_read_f16 must be 16-byte aligned");
     const uint64_t groups = (count + kReadPlaces - 1) / kReadPlaces * layer->kv_heads;
-    RBN_REQUIRE(groups < (1ull << 31), "too many places in rbn_kv_read_f16");
+    RBN_REQUIRE(groups < (1ull << 24), "too many places in rbn_kv_read_f16");  // a launch holds fewer than 2^32 threads
     RBN_ENTER(ctx);
     auto kernel = layer->format == RBN_KV_I8
                       ? (layer->head_dim == 128 ? kv_read_kernel<RBN_KV_I8, 128> : kv_read_kernel<RBN_KV_I8, 64>)

@@ -185,6 +185,21 @@ def test_null_descriptors_are_refused(lib):
             assert "null pointer" in message(lib, call), name
 
 
+def test_calls_of_too_many_workgroups_are_refused(lib):
+    """A launch holds fewer than 2^32 threads: the largest calls within the ranges of the single arguments do not fit."""
+    t, b, l = sound()
+    assert "aligned" in message(lib, calls(lib, t, b, l, out=0x20008)["read"])
+    b.max_tokens, l.kv_heads, t.rows = 1 << 18, 1024, 2048
+    assert "too much" in message(lib, calls(lib, t, b, l, heads=1024)["attend"])
+    assert "too much" in message(lib, calls(lib, t, b, l, heads=1024, max_new=2)["attend"])
+    assert message(lib, calls(lib, t, b, l, heads=1024)["store"]) == "context is NULL"
+    b.max_tokens = 1 << 13
+    assert message(lib, calls(lib, t, b, l, heads=1024)["attend"]) == "context is NULL"
+    assert message(lib, calls(lib, t, b, l, heads=1024, max_new=2)["attend"]) == "context is NULL"
+    assert "too many places" in message(lib, calls(lib, t, b, l, count=(1 << 20) + 1)["read"])
+    assert message(lib, calls(lib, t, b, l, count=(1 << 20) - 64)["read"]) == "context is NULL"
+
+
 def test_logprobs_refusals(lib):
     p = 0x10000
 
