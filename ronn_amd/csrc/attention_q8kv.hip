@@ -686,11 +686,9 @@ __device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int b
                     pm = load_agent(p);
                     pl = load_agent(p + 8 * NT);
                 }
-                float m = pm;
-                for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+                const float m = wave_max(pm);
                 const float k = pm == -INFINITY ? (pl != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(pm - m);
-                float den = k * pl;
-                for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+                const float den = wave_sum(k * pl);
                 s_weight[c][lane] = k;
                 if (lane == 0) s_den[c] = den;
             }

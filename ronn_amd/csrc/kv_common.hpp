@@ -4,6 +4,7 @@
 
 #include "common.hpp"
 #include "kv_index.h"
+#include "wave_ops.hpp"
 
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -52,18 +53,3 @@ __device__ __forceinline__ KvUnit kv_unit(const KvTableArgs &t, const KvBatchArg
     if (bad && threadIdx.x == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
     return r;
 }
-
-// Sum over the wave, and the inclusive prefix sum, on the DPP path; all lanes must be active.
-template <int CTRL, int ROWMASK>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWMASK, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan_i(int v) {
-    v = dpp_add<0x111, 0xf>(v);  // row_shr:1
-    v = dpp_add<0x112, 0xf>(v);  // row_shr:2
-    v = dpp_add<0x114, 0xf>(v);  // row_shr:4
-    v = dpp_add<0x118, 0xf>(v);  // row_shr:8
-    v = dpp_add<0x142, 0xa>(v);  // row_bcast15
-    return dpp_add<0x143, 0xc>(v);  // row_bcast31
-}
-__device__ __forceinline__ int wave_sum_i(int v) { return __builtin_amdgcn_readlane(wave_scan_i(v), 63); }

@@ -38,21 +38,6 @@ __device__ __forceinline__ float max_of(float m, float4 x) {
     return fmaxf(fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
 }
 
-template <int CTRL, int ROWMASK>
-__device__ __forceinline__ float dpp_max(float v) {  // v >= 0; lanes without a source take their own
-    const int w = __float_as_int(v);
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(w, w, CTRL, ROWMASK, 0xf, false)));
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = dpp_max<0x111, 0xf>(v);  // row_shr:1
-    v = dpp_max<0x112, 0xf>(v);  // row_shr:2
-    v = dpp_max<0x114, 0xf>(v);  // row_shr:4
-    v = dpp_max<0x118, 0xf>(v);  // row_shr:8
-    v = dpp_max<0x142, 0xa>(v);  // row_bcast15
-    v = dpp_max<0x143, 0xc>(v);  // row_bcast31
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-
 // x / scale, correctly rounded, from 1 / scale correctly rounded: the quotient's remainder is exact in one fma
 // and corrects it (Markstein 1990); f16 values and their scales are far from the ends of the f32 range.
 __device__ __forceinline__ float quotient(float x, float scale, float inverse) {

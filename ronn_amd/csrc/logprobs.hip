@@ -1,5 +1,6 @@
 // Log probabilities of given tokens, entropy and the top alternatives of rows of logits.
 #include "common.hpp"
+#include "wave_ops.hpp"
 
 namespace {
 
@@ -9,7 +10,7 @@ constexpr int kVecs = 4;                             // 16-byte loads of a threa
 constexpr int kGroups = kThreads / 8;                // groups of eight lanes, for the first threshold
 constexpr int kCandidates = 2048;
 constexpr int kMaxSegments = 16;
-constexpr int kMinSegment = 8192;
+constexpr int kMinSegment = 8192;                    // logits of one sweep
 constexpr int kTargetGroups = 512;
 static_assert(kGroups == 64, "a lane per group maximum");
 static_assert(kGroups >= RBN_TOP_MAX, "the top-th largest group maximum bounds the top-th largest logit");
@@ -38,31 +39,14 @@ __device__ __forceinline__ float lane_max(float v) {
 struct Stat {
     float m, s, w;
 };
-template <int CTRL, int ROWMASK, typename F>
-__device__ __forceinline__ float dpp_with(float v, float none, F f) {
-    return f(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWMASK, 0xf, false)));
-}
-// The wave's values brought together by f, in an order that is always the same; `none` leaves a value as it is.
-template <typename F>
-__device__ __forceinline__ float wave_all(float v, float none, F f) {
-    v = dpp_with<0x111, 0xf>(v, none, f);  // row_shr:1
-    v = dpp_with<0x112, 0xf>(v, none, f);  // row_shr:2
-    v = dpp_with<0x114, 0xf>(v, none, f);  // row_shr:4
-    v = dpp_with<0x118, 0xf>(v, none, f);  // row_shr:8
-    v = dpp_with<0x142, 0xa>(v, none, f);  // row_bcast15
-    v = dpp_with<0x143, 0xc>(v, none, f);  // row_bcast31
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-
 // The sets of all lanes as one: each is moved to the common maximum, then the sums are added.
 __device__ __forceinline__ Stat join(Stat a) {
-    const float m = wave_all(a.m, -INFINITY, [](float x, float y) { return fmaxf(x, y); });
-    auto sum = [](float v) { return wave_all(v, 0.0f, [](float x, float y) { return x + y; }); };
-    if (m == -INFINITY) return Stat{m, sum(a.s), 0.0f};  // nothing but -inf (s = 0) or NaN (s = NaN)
+    const float m = wave_max(a.m);
+    if (m == -INFINITY) return Stat{m, wave_sum(a.s), 0.0f};  // nothing but -inf (s = 0) or NaN (s = NaN)
     // a set that vanishes against the others (one of nothing but -inf among them) adds nothing, not 0 * -inf;
     // a NaN in its sum stays
     const float d = a.m - m, c = expf(d);
-    return Stat{m, sum(a.s * c), sum(c == 0.0f ? 0.0f : c * (a.w + d * a.s))};
+    return Stat{m, wave_sum(a.s * c), wave_sum(c == 0.0f ? 0.0f : c * (a.w + d * a.s))};
 }
 
 // The largest `top` of the n keys in cand, sorted, to out: each key's place is the number of larger ones
@@ -189,7 +173,7 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
             atomicAdd(&s_rank[lane], above);
             __syncthreads();
             // (equal but for those bits may stand in any order: the least of the first `want` it is)
-            return wave_all(s_rank[lane] < want ? s_group[lane] : INFINITY, INFINITY, [](float x, float y) { return fminf(x, y); });
+            return wave_min(s_rank[lane] < want ? s_group[lane] : INFINITY);
         };
         if (tid < held) s_cand[tid] = s_top[tid];
         if (first) {
@@ -283,7 +267,7 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
         // partial result of a segment: keys (padded with 0, which is below every key), then the sums
         constexpr size_t kPart = RBN_TOP_MAX * 8 + 16;
         char *mine = parts + (size_t)blockIdx.x * kPart;
-        if (tid < RBN_TOP_MAX)
+        if (tid < top)
             __hip_atomic_store(reinterpret_cast<uint64_t *>(mine) + tid, tid < want ? s_top[tid] : 0ull, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
         float *ms = reinterpret_cast<float *>(mine + RBN_TOP_MAX * 8);
@@ -302,8 +286,9 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
         if (!s_last) return;
         const char *all = parts + r * segments * kPart;
         static_assert(kMaxSegments * RBN_TOP_MAX <= kThreads, "one thread per key of a partial result");
-        if (tid < segments * RBN_TOP_MAX) {
-            const int p = tid / RBN_TOP_MAX, j = tid % RBN_TOP_MAX;
+        const int keys = segments * top;
+        if (tid < keys) {
+            const int p = tid / top, j = tid % top;
             s_cand[tid] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(all + p * kPart) + j, __ATOMIC_RELAXED,
                                             __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -318,12 +303,12 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
         st = join(part);
         __syncthreads();
         entries = min(top, vocab);
-        if (tid < segments * RBN_TOP_MAX && s_cand[tid] != 0) {
+        if (tid < keys && s_cand[tid] != 0) {
             const uint64_t key = s_cand[tid];
             int rank = 0;
             // (padding is below every key)
-#pragma unroll 16
-            for (int j = 0; j < segments * RBN_TOP_MAX; ++j) rank += s_cand[j] > key;
+#pragma unroll 8
+            for (int j = 0; j < keys; ++j) rank += s_cand[j] > key;
             if (rank < entries) s_top[rank] = key;
         }
         __syncthreads();
@@ -361,7 +346,7 @@ int rbn_token_logprobs_f32(rbn_ctx *ctx, const float *d_logits, uint64_t rows, u
     RBN_ENTER(ctx);
     // few rows: workgroups share a row, as long as each has enough to read
     uint64_t segments = kTargetGroups / rows;
-    const uint64_t most = vocab / kMinSegment;
+    const uint64_t most = (vocab + kMinSegment - 1) / kMinSegment;
     segments = segments < most ? segments : most;
     segments = segments < kMaxSegments ? segments : kMaxSegments;
     segments = segments > 1 ? segments : 1;
