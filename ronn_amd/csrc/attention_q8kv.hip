@@ -304,7 +304,11 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
 //  * The blocks of an item (token or unit, K/V head, up to 8 NT columns) go round the waves of the
 //    workgroups that share it.  How many share is decided on the device, where the lengths are: a share is
 //    what gives kTargetGroups shares in all, so that rows of any mix of lengths fill the chip evenly.
-//    The last workgroup of an item to finish joins the partial results in a fixed order.  Bound by the reading of the codes.
+//    The last workgroup of an item to finish joins the partial results in a fixed order.
+// Bound by the reading of the codes where there are many: 64 ragged rows up to 30000, 8 K/V heads, 377 MB: 71 us, 5.3 TB/s, 6.6
+// between start and join (non-temporal loads; 82 with ordinary ones); one row of 131000: 50.5 us.  With few by round trips: 1 row of
+// 1000, 20 heads: 10.3 us (task 2, q and pages 2.7, two blocks 2.7, publishing 1.8, joining 2.5).  A second block on its way per
+// wave changes nothing (71.6, 51.6, 10.6 us): a wave has some 1700 cycles of vector work per block.
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
 // Blocks a workgroup takes at least before another shares the item: 8 while that gives no more than a
@@ -737,6 +741,9 @@ __device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int b
 //    maximum lags behind by up to 2^8, and P is shifted up by 2^5: its parts reach at most 2^15, and the
 //    smallest step of f16 is 2^-25 or less of the largest weight.
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
+// Bound by the matrix instructions where there is much to do: five prompts of 268 to 1248 behind up to 1631 positions, 20 / 5 heads:
+// 58.4 us, 347 TFLOP/s (694 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
+// of the SIMD's two waves.  One prompt of 512, 20 heads: 24.3 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
 constexpr int kPromptThreads = 256;
 constexpr int kShift = 5;                 // log2 of what P is scaled up by
 constexpr int kPromptTargetGroups = 288;  // shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288)

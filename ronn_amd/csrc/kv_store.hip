@@ -289,7 +289,8 @@ __global__ __launch_bounds__(2 * HD) void kv_store_kernel(const float *__restric
 }
 
 // A workgroup has 64 places and a head, a lane a place: places are usually positions in a row, whose codes share the
-// cache lines of a page.  The values turn round in LDS and leave 16 bytes per thread, a place's head at a time.
+// cache lines of a page.  The values turn round in LDS and leave 16 bytes per thread, a place's head at a time
+// (3300 places, 20 heads: 14.3 us, 3.6 TB/s; 26 with a thread for eight dimensions of a place).
 constexpr int kReadThreads = 256, kReadPlaces = 64;
 
 template <int FMT, int HD>

@@ -80,7 +80,8 @@ __device__ __forceinline__ float4 load_once(const float *p) {
 //    instead, each a pass over the segment.
 // Bound by the reading of the logits; with few rows by latency.  1000 rows of 100003: 73 us, 5.5 TB/s with four workgroups on a
 // CU (8 waves per SIMD; 93 with the 66 registers of twice the loads in flight, 81 with those loads in 64; 100 with the next
-// sweep's loads ahead of the ranking: its registers spill).  16 rows of 32000: 11 us in segments of 8000, 12 of 4600.
+// sweep's loads ahead of the ranking: its registers spill).  16 rows of 32000: 8.4 us in four segments of 8000, a sweep
+// each (8.9 in six, 9.2 in eight, 11.3 in three of two sweeps).
 __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__restrict__ logits, int vocab, size_t pitch,
                                                                int segments, int seg_len,
                                                                const int32_t *__restrict__ target, int top,
