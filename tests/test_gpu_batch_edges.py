@@ -330,3 +330,18 @@ def test_logprobs_of_masked_rows(ctx, mask):
         x[7, [3, 4000, 8999]] = np.nan
         check_logprobs(ctx, x, rng.integers(0, vocab, 8), 20)
         check_logprobs(ctx, x[:, :vocab - 3], rng.integers(0, vocab - 3, 8), 32, pitch=vocab + 2, shift=1)
+
+
+def test_rows_of_one_block(ctx):
+    """A table with a single block per row: nothing to share, the block is unfinished until the very last position."""
+    rig = Rig(ctx, 6, 2, 64, "e4m3", rows=20, max_len=32, max_tokens=640, seed=2)
+    rng = np.random.default_rng(1)
+    q = rig.step(rng.integers(1, 20, 20))
+    for hint in (1, 5, 32):
+        rig.check_attention(q, hint, sample=60)
+    for kind in range(3):
+        q = rig.step([np.ones(20, int), 32 - rig.length, np.where(np.arange(20) % 3, 0, -1)][kind])
+        for hint in (1, 40):
+            rig.check_attention(q, hint) if len(q) else rig.attend(q, hint)
+    rig.check_cache()
+    assert ctx.device_flags() == 0
