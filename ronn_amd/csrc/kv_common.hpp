@@ -46,10 +46,3 @@ __device__ __forceinline__ float kv_decode(uint8_t c) {
     if (FMT == RBN_KV_I8) return (float)(int8_t)c;
     return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
 }
-
-__device__ __forceinline__ KvUnit kv_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, unsigned *flags) {
-    bool bad = false;
-    const KvUnit r = kv_resolve_unit(t, b, u, &bad);
-    if (bad && threadIdx.x == 0) atomicOr(flags, (unsigned)RBN_FLAG_KV_BAD_INDEX);
-    return r;
-}

@@ -78,13 +78,16 @@ KV_FN KvUnit kv_make_unit(const KvTableArgs &t, int tokens, int i, int row, int 
 }
 
 // Unit u of a batch (u below kv_max_units); *bad is set if there is one but what the batch says of it is not sound.
-// The loads do not wait for the counts.
-KV_FN KvUnit kv_resolve_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, bool *bad) {
+// The loads do not wait for the counts; ahead(i) is called while those of the unit's first token `i` (-1: not one of the
+// batch's places) are on their way.
+template <typename Ahead>
+KV_FN KvUnit kv_resolve_unit(const KvTableArgs &t, const KvBatchArgs &b, int u, bool *bad, Ahead ahead) {
     const int i = b.unit[u];
     const int tokens = b.count[0] < b.max_tokens ? b.count[0] : b.max_tokens;
     const int units = b.count[1] < b.max_tokens ? b.count[1] : b.max_tokens;
     const bool token = i >= 0 && i < b.max_tokens;  // (behind the count anything may stand there)
     const int row = token ? b.row[i] : -1, pos = token ? b.pos[i] : -1;
+    ahead(token ? i : -1);
     const bool known = row >= 0 && row < t.rows;
     KvUnit r = kv_make_unit(t, tokens, i, row, pos, known ? b.start[row] : -1, known ? b.start[row + 1] : -1);
     *bad = u < units && r.n == 0;

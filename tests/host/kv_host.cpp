@@ -14,7 +14,7 @@ int kv_unit_of(int rows, int max_blocks, int max_tokens, int32_t *start, int32_t
     KvTableArgs t{rows, max_blocks, 1, nullptr, nullptr, nullptr, nullptr};
     KvBatchArgs b{max_tokens, start, row, pos, nullptr, unit, count};
     bool bad = false;
-    const KvUnit r = kv_resolve_unit(t, b, u, &bad);
+    const KvUnit r = kv_resolve_unit(t, b, u, &bad, [](int) {});
     out[2] = r.n;
     if (r.n) {
         const int v[7] = {r.row, r.first, r.n, r.pos, r.row_first, r.row_pos, r.row_n};

@@ -62,6 +62,54 @@ def test_store_of_single_tokens_with_many_heads(ctx, heads, kv_heads, hd):
     assert ctx.device_flags() == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,fmt", [(4, 4, 128, "i8"), (40, 1, 64, "e4m3"), (17, 1, 128, "i8"), (6, 2, 64, "i8")])
+def test_store_of_decode_steps(ctx, heads, kv_heads, hd, fmt):
+    """Calls with no more tokens than rows: single tokens at every place of a block, now and then a few of one row over the end
+    of one, rows that end and start again."""
+    rows = 6
+    rig = Rig(ctx, heads, kv_heads, hd, fmt, rows=rows, max_len=160, max_tokens=rows, seed=heads)
+    rng = np.random.default_rng(heads)
+    for step in range(90):
+        new = np.ones(rows, int)
+        if step % 9 == 4:
+            new = np.zeros(rows, int)
+            new[rng.integers(rows)] = rng.integers(2, rows + 1)
+        elif step % 9 == 7:
+            new = rng.permutation([2, 2, 1, 1, 0, 0])
+        elif step % 20 == 19:
+            new[rng.integers(rows)] = -1
+        q = rig.step(new)
+        if step % 10 == 0:
+            rig.check_attention(q, int(new.max()), sample=6)
+    rig.check_cache()
+    assert ctx.device_flags() == 0
+
+
+def test_store_of_a_decode_step_saturates_flags_and_checks(ctx):
+    rig = Rig(ctx, 2, 1, 64, "i8", rows=4, max_tokens=4, seed=3)
+    rig.step([1, 1, 1, 1])
+    x = rig.qkv(4)
+    x[0, 2 * 64 + 64 + 3], x[1, 2 * 64 + 64 + 5], x[2, 2 * 64 + 64 + 7] = np.nan, 1e9, -np.inf      # in v
+    rig.step([1, 1, 1, 1], x)
+    assert ctx.device_flags() == _lib.FLAG_KV_NONFINITE
+    rig.check_cache()
+    # slots without a page: flagged; units that are none: left out
+    before = [b.download(np.uint8, b.nbytes) for b in rig.cache.buffers[0]]
+    rig.cache.plan(rig.d_new)
+    d_qkv = ctx.to_device(rig.qkv(4))
+    rig.cache.d_unit.upload(np.array([-1, 4, 2 ** 31 - 1, -2 ** 31], np.int32))
+    rig.cache.store(0, d_qkv, 2, 1e4, rig.d_q)
+    assert ctx.device_flags() == _lib.FLAG_KV_BAD_INDEX
+    for b, was in zip(rig.cache.buffers[0], before):
+        assert (b.download(np.uint8, b.nbytes) == was).all()
+    rig.cache.d_unit.upload(np.arange(4, dtype=np.int32))
+    rig.cache.d_slot.upload(np.array([-1, 2 ** 31 - 1, -1, -1], np.int32))
+    rig.cache.store(0, d_qkv, 2, 1e4, rig.d_q)
+    assert ctx.device_flags() == _lib.FLAG_KV_BAD_INDEX
+    for i in (0, 1, 4, 5):                         # no page and no scale
+        assert (rig.cache.buffers[0][i].download(np.uint8, rig.cache.buffers[0][i].nbytes) == before[i]).all()
+
+
 def test_read_of_any_places(ctx):
     """Places in any order, the same one twice, open and full blocks and none, over several workgroups."""
     rig = Rig(ctx, 3, 3, 64, "e4m3", rows=5, max_tokens=512, seed=4)
