@@ -337,11 +337,13 @@ struct TokenShared {
     int last;
 };
 
-template <int FMT, int HD, int NT, bool PER_TOKEN>
-__device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int block, const float *__restrict__ q,
-                                              const KvTableArgs &t, const KvBatchArgs &b, const KvLayerArgs &l, int heads,
-                                              int tiles, int max_shares, int max_columns, float *__restrict__ partials,
-                                              unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
+// A share of an item, the one that deal_it() says.  Of the partial results' place every share takes room for PART_NT tiles
+// of columns.
+template <int FMT, int HD, int NT, int PART_NT, typename Deal>
+__device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal deal_it, const float *__restrict__ q,
+                                            const KvTableArgs &t, const KvLayerArgs &l, int heads, int group, int each, int rest,
+                                            int kvh, int cg, float *__restrict__ partials, unsigned *__restrict__ tickets,
+                                            float *__restrict__ out, unsigned *flags) {
     constexpr int KK = HD / 32;   // k steps of the scores
     constexpr int DT = HD / 16;   // tiles of dimensions of the output
     constexpr int LD = HD / 32;   // 16-byte loads per lane of 32 keys, K and V each
@@ -357,11 +359,7 @@ __device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int b
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane: branches on it are scalar
     const int c16 = lane & 15, c8 = lane & 7, g = lane >> 4;
-    const int group = heads / l.kv_heads;
-    // this workgroup's task: an item (token or unit, K/V head, tile of columns) and a share of its blocks
-    const int each = l.kv_heads * tiles, rest = block % each, kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
-    const Task task = deal<PER_TOKEN>(t, b, block, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare,
-                                      2 * kMinShare, flags, [](const KvUnit &u) { return u.pos / kKvBlock + 1; });
+    const Task task = deal_it();
     if (task.entry < 0) return;
     const int row = task.unit.row, pos = task.unit.pos, first = task.unit.first, n = task.unit.n;
     const int split = task.split, shares = task.shares;
@@ -623,7 +621,7 @@ __device__ __forceinline__ void attend_tokens(TokenShared<HD, NT> &shared, int b
     __syncthreads();
     const int ncols = min(8 * NT, cols - cg * 8 * NT);
     const int slot = task.entry * each + rest;  // used by shared items only
-    float *part = partials + ((size_t)task.place * each + (size_t)rest * shares) * partial_floats<HD, NT>();
+    float *part = partials + ((size_t)task.place * each + (size_t)rest * shares) * partial_floats<HD, PART_NT>();
     auto write_out = [&](int c, int d, v4f num, float den) {
         const int col = cg * 8 * NT + c, token = col / group;
         const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
@@ -1201,19 +1199,31 @@ __device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int blo
                 make_float4(o[nt][4 * r4] * inv, o[nt][4 * r4 + 1] * inv, o[nt][4 * r4 + 2] * inv, o[nt][4 * r4 + 3] * inv);
 }
 
+// The task of workgroup `block` of those for few columns: an item (token or unit, K/V head, tile of columns) and a share
+// of its blocks.
+template <bool PER_TOKEN>
+__device__ __forceinline__ Task deal_tokens(const KvTableArgs &t, const KvBatchArgs &b, int block, int group, int max_columns,
+                                            int each, int max_shares, unsigned *flags) {
+    return deal<PER_TOKEN>(t, b, block, group, 0, max_columns, each, max_shares, kTargetGroups, kMinShare, 2 * kMinShare, flags,
+                           [](const KvUnit &u) { return u.pos / kKvBlock + 1; });
+}
+
 // One token per row.
 template <int FMT, int HD, int NT>
 __global__ __launch_bounds__(kTokenThreads, NT == 1 ? 3 : 2) void attention_token_kernel(
     const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int tiles, int max_shares,
     float *__restrict__ partials, unsigned *__restrict__ tickets, float *__restrict__ out, unsigned *flags) {
     __shared__ __attribute__((aligned(16))) TokenShared<HD, NT> shared;
-    attend_tokens<FMT, HD, NT, true>(shared, blockIdx.x, q, t, b, l, heads, tiles, max_shares, INT32_MAX, partials, tickets,
-                                     out, flags);
+    const int group = heads / l.kv_heads, each = l.kv_heads * tiles, rest = blockIdx.x % each;
+    const int kvh = rest % l.kv_heads, cg = rest / l.kv_heads;
+    auto deal_it = [&]() { return deal_tokens<true>(t, b, blockIdx.x, group, INT32_MAX, each, max_shares, flags); };
+    attend_task<FMT, HD, NT, NT>(shared, deal_it, q, t, l, heads, group, each, rest, kvh, cg, partials, tickets, out, flags);
 }
 
 // Any number of tokens per row: the first `prompts` workgroups are for rows with more than kFewColumns columns, the
-// others for the rest; one launch, so that a batch of both kinds runs at the same time and one of a single kind does
-// not wait for a launch that finds nothing to do (4.5 us).
+// others for the rest (a single tile where eight columns do: 64 rows of 4000, 4 heads per K/V head, called as if they had more
+// than a token each: 136 us with two, 113 with one, 97 as what they are); one launch, so that a batch of both kinds runs at the same time and one of a
+// single kind does not wait for a launch that finds nothing to do (4.5 us).
 template <int FMT, int HD>
 __global__ __launch_bounds__(kPromptThreads, 2) void attention_batch_kernel(
     const float *__restrict__ q, KvTableArgs t, KvBatchArgs b, KvLayerArgs l, int heads, int prompts, int prompt_shares,
@@ -1226,14 +1236,26 @@ __global__ __launch_bounds__(kPromptThreads, 2) void attention_batch_kernel(
     static_assert(kTokenThreads == kPromptThreads, "both kinds of workgroup are of one launch");
     __shared__ union {
         TokenShared<HD, NT> tokens;
+        TokenShared<HD, 1> few;
         PromptShared<HD> prompts;
     } shared;
-    if ((int)blockIdx.x < prompts)
+    if ((int)blockIdx.x < prompts) {
         attend_prompts<FMT, HD>(shared.prompts, blockIdx.x, q, t, b, l, heads, prompt_shares, kFewColumns + 1, partials,
                                 tickets, out, flags);
+        return;
+    }
+    const int block = blockIdx.x - prompts, group = heads / l.kv_heads, each = l.kv_heads, rest = block % each;
+    const Task task = deal_tokens<false>(t, b, block, group, kFewColumns, each, token_shares, flags);
+    if (task.entry < 0) return;
+    float *token_partials = partials + kPromptPartials;
+    unsigned *token_tickets = tickets + RBN_ATTENTION_ITEMS;
+    auto dealt = [&]() { return task; };
+    if (task.unit.n * group <= 8)
+        attend_task<FMT, HD, 1, NT>(shared.few, dealt, q, t, l, heads, group, each, rest, rest, 0, token_partials, token_tickets,
+                                    out, flags);
     else
-        attend_tokens<FMT, HD, NT, false>(shared.tokens, blockIdx.x - prompts, q, t, b, l, heads, 1, token_shares,
-                                          kFewColumns, partials + kPromptPartials, tickets + RBN_ATTENTION_ITEMS, out, flags);
+        attend_task<FMT, HD, NT, NT>(shared.tokens, dealt, q, t, l, heads, group, each, rest, rest, 0, token_partials,
+                                     token_tickets, out, flags);
 }
 
 // The most workgroups that may share an item, as far as there are tickets; how many do is decided on the device,
