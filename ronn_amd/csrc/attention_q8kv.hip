@@ -740,7 +740,7 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
 //    smallest step of f16 is 2^-25 or less of the largest weight.
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 // Bound by the matrix instructions where there is much to do: five prompts of 268 to 1248 behind up to 1631 positions, 20 / 5 heads:
-// 58.4 us, 347 TFLOP/s (694 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
+// 59 us, 343 TFLOP/s (686 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
 // of the SIMD's two waves.  One prompt of 512, 20 heads: 24.3 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
 constexpr int kPromptThreads = 256;
 constexpr int kShift = 5;                 // log2 of what P is scaled up by
