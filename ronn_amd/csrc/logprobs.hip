@@ -75,7 +75,7 @@ __device__ __forceinline__ float4 load_once(const float *p) {
 //    than twice `top`) go to a list in LDS, which is ranked by counting.  Later sweeps add what exceeds the
 //    list's last entry (their indices are higher, so equals lose).  A sweep with too many of them is looked at once
 //    more, with a bound of its own and no more equals than can count (1000 rows of 100003 with all but 20 logits at one
-//    value: 90 us, before that 2.4 ms by the way below; in ascending order 0.77 ms).
+//    value: 85 us, before that 2.4 ms by the way below; in ascending order 0.76 ms).
 //  * Where the list overflows even so, or comes out short (NaN), the segment's alternatives are found one by one
 //    instead, each a pass over the segment.
 // Bound by the reading of the logits; with few rows by latency.  1000 rows of 100003: 73 us, 5.5 TB/s with four workgroups on a
@@ -95,7 +95,8 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
     __shared__ uint64_t s_best[kWaves];
     __shared__ float s_group[kGroups];
     __shared__ int s_rank[kGroups];
-    __shared__ int s_count, s_first, s_last;
+    __shared__ int s_equals[kWaves];
+    __shared__ int s_count, s_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in every lane
     const size_t r = blockIdx.x / segments;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
             gm = lane_max<0x141>(gm);         // row_half_mirror: the other four of the eight
             if ((lane & 7) == 0) s_group[tid >> 3] = gm;
             if (tid < kGroups) s_rank[tid] = 0;
-            if (tid == 0) s_count = entries, s_first = INT32_MAX;
+            if (tid == 0) s_count = entries;
             __syncthreads();
             // the maxima as unsigned numbers in the same order, the last six bits for their places: all differ.  Each
             // wave compares them with eight of them.
@@ -203,24 +204,40 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(const float *__re
         const int so_far = min(n, (sweep == sweeps - 1 ? n : head + 4 * kThreads * kVecs * (sweep + 1)));
         if (found > kCandidates) {
             // too many at the bound (masked logits, say) or above it (a row in ascending order): the sweep once more, with
-            // the bound that it gives itself, and of equals at the bound those from the first on that can count if
-            // nothing else stands among them
+            // the bound that it gives itself: what is above it, and the first `want` equals in the order of their indices
+            // (a wave takes an eighth of the sweep; what the waves before it have gives its equals their ranks).  `want`
+            // logits of the sweep are at that bound or above, so the list is short of nothing that counts.
             __syncthreads();
             bound = fmaxf(bound, threshold(held));
             const int from = first ? lo : vec_lo + 4 * kThreads * kVecs * sweep, to = lo + so_far;
+            const int each = (to - from + kWaves - 1) / kWaves;
+            const int mine = min(from + wave * each, to), behind = min(mine + each, to);
             if (tid < held) s_cand[tid] = s_top[tid];
-#pragma unroll 1
-            for (int i = from + tid; i < to; i += kThreads)
-                if (x[i] == bound) {
-                    atomicMin(&s_first, i);
-                    break;
-                }
+            float a[4];
+            auto load = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = i + 64 * j + lane < behind ? x[i + 64 * j + lane] : NAN;
+            };
+            int rank = 0;
+            for (int i = mine; i < behind && rank < want; i += 256) {  // (more than `want` need not be told apart)
+                load(i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) rank += __popcll(__ballot(a[j] == bound));
+            }
+            if (lane == 0) s_equals[wave] = rank;
             __syncthreads();
-            const int near = s_first < INT32_MAX - RBN_TOP_MAX ? s_first + want : s_first;
-#pragma unroll 1
-            for (int i = from + tid; i < to; i += kThreads) {
-                const float a = x[i];
-                if (a > bound || (a == bound && i < near)) put(a, i);
+            rank = 0;
+            for (int w = 0; w < wave; ++w) rank += s_equals[w];
+            for (int i = mine; i < behind; i += 256) {
+                load(i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned long long equals = __ballot(a[j] == bound);
+                    const int before =
+                        __builtin_amdgcn_mbcnt_hi((unsigned)(equals >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)equals, 0));
+                    if (a[j] > bound || (a[j] == bound && rank + before < want)) put(a[j], i + 64 * j + lane);
+                    rank += __popcll(equals);
+                }
             }
             __syncthreads();
             found = s_count;
