@@ -52,6 +52,14 @@ __device__ __forceinline__ float other_half(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // row_ror:8
 }
 
+// The maximum of the four lanes of a column, sixteen apart.
+__device__ __forceinline__ float column_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 __device__ __forceinline__ float load_agent(const float *p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -296,11 +304,14 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
 //  * The codes are exact in f16.  q (scaled to |q| < 2 by a power of two for each column) and the
 //    probabilities go in as hi + lo f16 pairs, 22 bits: of the 16 columns of a tile, 0-7 carry the hi
 //    parts of eight (token, head) columns and 8-15 their lo parts, so one instruction does both.
+//  * A column's probabilities of a block are scaled by a power of two that puts the largest of them into [2^14, 2^15): f16's
+//    smallest step is 2^-38 of that, so a block far below the maximum keeps its 22 bits and many of them add up to what they
+//    should.  The scale comes out with V's, when the block's output is added.
 //  * A page is laid out as the instructions read it: a lane's operand bytes are consecutive, a wave's
 //    loads are whole cache lines, and P^T comes out of the score tiles already in operand order
 //    (slot e of lane group g is key 16 (e/4) + 4 g + e%4; V's layout follows).
-//  * The running maximum is shared by the four lanes of a column and moves only when a score exceeds it
-//    by 8 (powers of two): the usual block costs no cross-lane step.  Sums are per lane until the end.
+//  * The running maximum, in whole powers of two, moves only when a score exceeds it by 8 of them: the usual block does not
+//    touch the output but to add to it.  Sums are per lane until the end.
 //  * The blocks of an item (token or unit, K/V head, up to 8 NT columns) go round the waves of the
 //    workgroups that share it.  How many share is decided on the device, where the lengths are: a share is
 //    what gives kTargetGroups shares in all, so that rows of any mix of lengths fill the chip evenly.
@@ -472,6 +483,7 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
     auto attend = [&](const v4f (&s)[NT][2], auto value, float kscale, float vscale, int t0) {
         const bool masked = t0 + kKvBlock - 1 > pos;
         v8h pf[NT];
+        float vs_up[NT];
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
             const float f = kscale * col_scale[ct];
@@ -483,9 +495,8 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
                 if (masked) x[e] = t0 + 16 * (e >> 2) + 4 * g + (e & 3) <= col_pos[ct] ? x[e] : -INFINITY;
                 m = fmaxf(m, x[e]);
             }
+            m = floorf(column_max(m));
             if (__any(m > run_max[ct] + 8.0f)) {
-                m = fmaxf(m, __shfl_xor(m, 16));
-                m = fmaxf(m, __shfl_xor(m, 32));
                 const float top = fmaxf(run_max[ct], m);
                 const float corr = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max[ct] - top);
                 run_max[ct] = top;
@@ -493,14 +504,20 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[ct][d] *= corr;
             }
-            const float ref = run_max[ct] == -INFINITY ? 0.0f : run_max[ct];  // nothing seen yet: p = 0
+            // the block's weights on a scale of their own, the largest in [2^14, 2^15), and that scale in units of the output
+            const bool none = m == -INFINITY;
+            const float unit = none ? 0.0f : m - 14.0f;
+            const float up = none ? 0.0f : __builtin_amdgcn_exp2f(unit - run_max[ct]);
+            float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = __builtin_amdgcn_exp2f(x[e] - ref);
-                run_sum[ct] += p;
+                const float p = __builtin_amdgcn_exp2f(x[e] - unit);
+                sum += p;
                 const _Float16 hi = (_Float16)p, lo = (_Float16)(p - (float)hi);
                 pf[ct][e] = c16 < 8 ? hi : lo;
             }
+            run_sum[ct] = fmaf(sum, up, run_sum[ct]);
+            vs_up[ct] = vscale * up;
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -509,7 +526,7 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
             for (int ct = 0; ct < NT; ++ct) {
                 const v4f z = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[ct][d][r] = fmaf(z[r], vscale, o[ct][d][r]);
+                for (int r = 0; r < 4; ++r) o[ct][d][r] = fmaf(z[r], vs_up[ct], o[ct][d][r]);
             }
         }
     };
@@ -734,16 +751,21 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
 //    workgroup take four in a row and share the keys and values, which the workgroup converts
 //    once to f16 in LDS, in operand order: every operand read is one conflict-free 16-byte read per lane.
 //  * q and P in f16 as hi + lo, two instructions each (a tile has 32 columns of its own here).  V's scale goes
-//    into P; the output is kept in units of a power of two near the scales so far.  Scales within [2^-4, 4)
-//    of the unit use it as it is, others move it (the store's scales span 2^-32 .. 2^9), the running
-//    maximum lags behind by up to 2^8, and P is shifted up by 2^5: its parts reach at most 2^15, and the
-//    smallest step of f16 is 2^-25 or less of the largest weight.
+//    into P, as its logarithm in the exponent (off by 2^-20 of it at most, at 2^-32); the output is kept in units of a
+//    power of two near the scales so far.  Scales within [2^-4, 4) of the unit use it as it is, others move it (the
+//    store's scales span 2^-32 .. 2^9), the running maximum lags behind by up to 2^4, and P is shifted up by 2^9: its
+//    parts reach at most 2^15.  Where V's scale is the unit, a weight is off by up to 2^-34 of the largest (half of f16's
+//    smallest step), so L keys far below it by up to L 2^-34 of V's largest together: 128 u with 131072 keys, u = 2^-24, a
+//    third of what sums of as many terms round by.  (The output is summed up inside the matrix instructions, so a block's
+//    weights cannot have a scale of their own as they have above.)
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 // Bound by the matrix instructions where there is much to do: five prompts of 268 to 1248 behind up to 1631 positions, 20 / 5 heads:
 // 59 us, 343 TFLOP/s (686 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
 // of the SIMD's two waves.  One prompt of 512, 20 heads: 24.3 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
 constexpr int kPromptThreads = 256;
-constexpr int kShift = 5;                 // log2 of what P is scaled up by
+// Powers of two that the running maximum may lag behind, and log2 of what P is scaled up by.  A lag moves the output less often (five
+// ragged prompts: 59.6 us with 8, 60.4 with 4, 60.9 with 3) and leaves P as many bits less.
+constexpr int kLag = 4, kShift = 13 - kLag;
 constexpr int kPromptTargetGroups = 288;  // shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288)
 // blocks a workgroup takes at least before another shares the tile: partial results cost some 10 us to write, wait for
 // and join, a block 0.75 (one prompt of 512, 20 heads: 27.2 us with 4, 25.5 with 8, 24.7 with 12, 27.9 with 16 or none shared)
@@ -968,7 +990,7 @@ __device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int blo
             m = max_of(s);
         }
         m *= f;
-        if (__any(m > run_max + 8.0f)) {
+        if (__any(m > run_max + (float)kLag)) {
             m = fmaxf(m, __shfl_xor(m, 32));
             const float mx = fmaxf(run_max, m);
             const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
