@@ -14,6 +14,7 @@ with the same weights over the paged 8-bit cache (kvcache.py), with log probabil
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import dataclasses
 import time
@@ -328,7 +329,8 @@ class BatchDecoder:
     A row is the place of one sequence (0 .. rows - 1): start() puts prompts into free rows, step() advances every
     running row by its greedy token, finish() frees rows.  score() gives the log probabilities of given tokens.
     pages: pages of 32 positions shared by the rows (0: enough for every row at cfg.max_seq); max_tokens: the most
-    tokens of one call; top: alternatives that come with every token (1 to 32)."""
+    tokens of one call; top: alternatives that come with every token (1 to 32).  A call that is refused changes nothing; where one
+    fails on the way (a launch, say), the rows that it had advanced on the device end and are free again."""
 
     LOGIT_ROWS = 256    # rows of logits computed at a time when prompts are scored
 
@@ -362,6 +364,7 @@ class BatchDecoder:
         self._len = np.zeros(rows, dtype=np.int64)     # host copies of what the device holds
         self._free = pages
         self._next = {}                                # running rows: their NextToken
+        self._lost = False                             # whether they can no longer be trusted
 
     # -- queueing ------------------------------------------------------------------------------------
     def _forward(self, M: int, max_new: int):
@@ -416,8 +419,13 @@ class BatchDecoder:
         return raw[:M].view(np.float32).copy(), raw[R:R + M].view(np.float32).copy(), tok.copy(), lps.copy()
 
     # -- what the host knows before it queues anything --------------------------------------------------
-    def _admit(self, new: dict):
-        """Checks and books `new` tokens per row, so that no row is refused on the device."""
+    def _check_known(self):
+        if self._lost:
+            raise RuntimeError("an earlier call failed and what the device holds is unknown")
+
+    def _check_room(self, new: dict) -> int:
+        """Refuses `new` tokens per row that the device would refuse; returns how many pages they need."""
+        self._check_known()
         total = sum(new.values())
         if total > self.max_tokens:
             raise ValueError("%d tokens in one call: max_tokens is %d" % (total, self.max_tokens))
@@ -429,23 +437,44 @@ class BatchDecoder:
             need += blocks(self._len[r] + n) - blocks(self._len[r])
         if need > self._free:
             raise ValueError("%d pages are needed, %d are free" % (need, self._free))
-        self._free -= need
-        for r, n in new.items():
-            self._len[r] += n
+        return need
+
+    @contextlib.contextmanager
+    def _admitted(self, new: dict):
+        """Books `new` tokens per row for the work queued inside.  Where that fails, the host's copies are brought in line with
+        the device, and rows that had advanced there, whose new positions may hold nothing, end."""
+        before, need = self._len.copy(), self._check_room(new)
+        try:
+            self._upload_counts(new)
+            self._free -= need
+            for r, n in new.items():
+                self._len[r] += n
+            yield sum(new.values())
+        except BaseException:
+            try:
+                self._len = self.cache.lengths().astype(np.int64)
+                self._free = self.cache.free_pages()
+                ended = [r for r in new if self._len[r] != before[r]]
+                if ended:
+                    self._release(ended)
+                for r in ended:
+                    self._next.pop(r, None)
+            except Exception:
+                self._lost = True
+            raise
+
+    def _upload_counts(self, new: dict):
         counts = np.zeros(self.rows, dtype=np.int32)
         for r, n in new.items():
             counts[r] = n
         self.d_new.upload(counts)
-        return total
 
     def _release(self, rows):
-        counts = np.zeros(self.rows, dtype=np.int32)
+        self._upload_counts({r: -1 for r in rows})
+        self.cache.plan(self.d_new)
         for r in rows:
-            counts[r] = -1
             self._free += -(-int(self._len[r]) // _lib.KV_BLOCK)
             self._len[r] = 0
-        self.d_new.upload(counts)
-        self.cache.plan(self.d_new)
 
     def _prompts(self, prompts: dict) -> dict:
         out = {}
@@ -471,18 +500,19 @@ class BatchDecoder:
     def start(self, prompts: dict) -> dict:
         """Puts prompts (row -> token ids) into free rows; returns row -> NextToken."""
         prompts = self._prompts(prompts)
-        self._admit({r: ids.size for r, ids in prompts.items()})
         ids = np.concatenate(list(prompts.values()))
-        self.tokens.upload(ids)
-        self._forward(ids.size, max(p.size for p in prompts.values()))
-        # the last token of each prompt
-        pitch = self.ctx.act_pitch(self.cfg.hidden)
-        ends = np.cumsum([p.size for p in prompts.values()]) - 1
-        for i, e in enumerate(ends):
-            for src, dst, n in zip(self.acts, self.last, (pitch, 4, 4)):
-                check(self.lib.rbn_d2d(self.ctx.handle, dst.ptr + i * n, src.ptr + int(e) * n, n))
-        self._logprobs(self.last, 0, len(ends), False)
-        return self._took(list(prompts), *self._fetch(len(ends))[1:])
+        with self._admitted({r: p.size for r, p in prompts.items()}):
+            self.tokens.upload(ids)
+            self._forward(ids.size, max(p.size for p in prompts.values()))
+            # the last token of each prompt
+            pitch = self.ctx.act_pitch(self.cfg.hidden)
+            ends = np.cumsum([p.size for p in prompts.values()]) - 1
+            for i, e in enumerate(ends):
+                for src, dst, n in zip(self.acts, self.last, (pitch, 4, 4)):
+                    check(self.lib.rbn_d2d(self.ctx.handle, dst.ptr + i * n, src.ptr + int(e) * n, n))
+            self._logprobs(self.last, 0, len(ends), False)
+            got = self._fetch(len(ends))
+        return self._took(list(prompts), *got[1:])
 
     def _took(self, rows, entropy, tok, lps) -> dict:
         got = {r: NextToken(int(tok[i, 0]), float(lps[i, 0]), float(entropy[i]), tok[i], lps[i]) for i, r in enumerate(rows)}
@@ -495,20 +525,29 @@ class BatchDecoder:
         rows = sorted(self._next)
         if not rows:
             raise ValueError("no row is running")
-        M = self._admit({r: 1 for r in rows})
-        self.tokens.upload(np.array([self._next[r].token for r in rows], dtype=np.int32))
+        new, M = {r: 1 for r in rows}, len(rows)
         if use_graph and M not in self._graphs:
-            self.ctx.graph_begin()
-            try:
+            self._check_room(new)
+            self._graphs[M] = self._capture_step(M)
+        with self._admitted(new):
+            self.tokens.upload(np.array([self._next[r].token for r in rows], dtype=np.int32))
+            if use_graph:
+                self.ctx.graph_launch(self._graphs[M])
+            else:
                 self._queue_step(M)
-            finally:
-                g = self.ctx.graph_end()
-            self._graphs[M] = g
-        if use_graph:
-            self.ctx.graph_launch(self._graphs[M])
-        else:
+            got = self._fetch(M)
+        return self._took(rows, *got[1:])
+
+    def _capture_step(self, M: int):
+        self.ctx.graph_begin()
+        try:
             self._queue_step(M)
-        return self._took(rows, *self._fetch(M)[1:])
+        except BaseException:
+            # the capture has to end; a graph of a part of the step is of no use
+            with contextlib.suppress(_lib.RbnError):
+                self.ctx.graph_destroy(self.ctx.graph_end())
+            raise
+        return self.ctx.graph_end()
 
     def _queue_step(self, M: int):
         self._forward(M, 1)
@@ -519,6 +558,7 @@ class BatchDecoder:
         rows = [rows] if isinstance(rows, (int, np.integer)) else list(rows)
         if len(set(rows)) != len(rows) or any(r not in self._next for r in rows):
             raise ValueError("rows %s are not all running" % rows)
+        self._check_known()
         self._release(rows)
         for r in rows:
             del self._next[r]
@@ -528,21 +568,21 @@ class BatchDecoder:
         tokens 1 .. and the entropy before each of them: row -> (logprobs [n-1], entropies [n-1]).  The rows are
         free again afterwards."""
         prompts = self._prompts(prompts)
-        self._admit({r: ids.size for r, ids in prompts.items()})
         ids = np.concatenate(list(prompts.values()))
         # token i is followed by token i + 1 of its own prompt; the last one has no target
         targets = np.concatenate([np.append(p[1:], -1) for p in prompts.values()]).astype(np.int32)
-        self.tokens.upload(ids)
-        self.targets.upload(targets)
-        self._forward(ids.size, max(p.size for p in prompts.values()))
         lp, ent = [], []
-        for at in range(0, ids.size, self.logit_rows):
-            n = min(self.logit_rows, ids.size - at)
-            self._logprobs(self.acts, at, n, True)
-            got = self._fetch(n)
-            lp.append(got[0])
-            ent.append(got[1])
-        self._release(list(prompts))
+        with self._admitted({r: p.size for r, p in prompts.items()}):
+            self.tokens.upload(ids)
+            self.targets.upload(targets)
+            self._forward(ids.size, max(p.size for p in prompts.values()))
+            for at in range(0, ids.size, self.logit_rows):
+                n = min(self.logit_rows, ids.size - at)
+                self._logprobs(self.acts, at, n, True)
+                got = self._fetch(n)
+                lp.append(got[0])
+                ent.append(got[1])
+            self._release(list(prompts))
         lp, ent = np.concatenate(lp), np.concatenate(ent)
         out, at = {}, 0
         for r, p in prompts.items():
