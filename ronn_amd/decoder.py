@@ -27,6 +27,10 @@ from .device import Context, DeviceBuffer
 from .kvcache import PagedKVCache
 
 
+class _AsHeads(int):
+    """A number of K/V heads that nobody gave: it stays that of the query heads."""
+
+
 @dataclasses.dataclass
 class DecoderConfig:
     layers: int = 24
@@ -40,9 +44,15 @@ class DecoderConfig:
     rope_theta: float = 10000.0
     kv_heads: int = 0       # K/V heads; 0: as many as query heads.  Fewer are served by BatchDecoder only
 
+    def __setattr__(self, name, value):
+        if name == "kv_heads" and (not value or isinstance(value, _AsHeads)):
+            value = _AsHeads(self.heads)
+        object.__setattr__(self, name, value)
+        if name == "heads" and isinstance(vars(self).get("kv_heads"), _AsHeads):
+            self.kv_heads = 0
+
     def __post_init__(self):
-        self.kv_heads = self.kv_heads or self.heads
-        if self.kv_heads < 0 or self.heads % self.kv_heads:
+        if self.kv_heads < 0 or (self.kv_heads and self.heads % self.kv_heads):
             raise ValueError("heads (%d) must be a multiple of kv_heads (%d)" % (self.heads, self.kv_heads))
 
     @property
