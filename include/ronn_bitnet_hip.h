@@ -450,7 +450,8 @@ int rbn_kv_plan(rbn_ctx *ctx, const rbn_kv_table *table, const int32_t *d_new,
  * head_dim] f32 = (q | k | v), not modified.  Rotates the pairs (i, i + head_dim/2) of q and k by the
  * angle pos * theta^(-2i/head_dim), evaluated in 64 bits; rotated q goes to d_q [max_tokens, heads *
  * head_dim] f32 (16-byte aligned), k and v into the cache.  Rows of d_q behind the last token are left alone.
- * heads is a multiple of kv_heads, at most 1024. */
+ * heads is a multiple of kv_heads, at most 1024; theta is positive, with max_blocks *
+ * RBN_KV_BLOCK * theta^(2/head_dim - 1) below 2^50. */
 int rbn_rope_kv_store_q8(rbn_ctx *ctx, const float *d_qkv, const rbn_kv_table *table,
                          const rbn_kv_batch *batch, const rbn_kv_layer *layer, uint64_t heads,
                          float theta, float *d_q);

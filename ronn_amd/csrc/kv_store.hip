@@ -444,6 +444,9 @@ int rbn_rope_kv_store_q8(rbn_ctx *ctx, const float *d_qkv, const rbn_kv_table *t
                 "heads (%llu) must be a multiple of kv_heads (%u), at most 1024", (unsigned long long)heads,
                 layer->kv_heads);
     RBN_REQUIRE(theta > 0.0f && theta <= 3.4e38f, "theta must be positive and finite");
+    // rotation() holds the whole quarter turns in 51 bits (theta < 1 has pairs that turn more than a radian per position)
+    RBN_REQUIRE((double)table->max_blocks * RBN_KV_BLOCK * exp2(-(1.0 - 2.0 / layer->head_dim) * log2((double)theta)) < 0x1p50,
+                "theta %g is too small for rows of %llu blocks", (double)theta, (unsigned long long)table->max_blocks);
     RBN_ENTER(ctx);
     const unsigned groups = (unsigned)kv_max_units(batch->max_tokens, table->rows) * layer->kv_heads;
     static_assert((RBN_KV_MAX_TOKENS / RBN_KV_BLOCK + 2ull * RBN_KV_MAX_ROWS) * 1024 * 256 < 1ull << 32, "threads of a launch");
