@@ -489,14 +489,16 @@ class BatchDecoder:
     def _prompts(self, prompts: dict) -> dict:
         out = {}
         for r, ids in sorted(prompts.items()):
-            ids = np.ascontiguousarray(ids, dtype=np.int32)
+            ids = np.asarray(ids)
             if not 0 <= r < self.rows:
                 raise ValueError("row %d is outside [0, %d)" % (r, self.rows))
             if r in self._next:
                 raise ValueError("row %d is running" % r)
             if ids.ndim != 1 or ids.size == 0:
                 raise ValueError("a prompt must be a non-empty vector of token ids")
-            out[r] = ids
+            if not (ids.min() >= 0 and ids.max() < self.cfg.vocab):
+                raise ValueError("the prompt of row %d has token ids outside [0, %d)" % (r, self.cfg.vocab))
+            out[r] = np.ascontiguousarray(ids, dtype=np.int32)
         if not out:
             raise ValueError("no prompts")
         return out

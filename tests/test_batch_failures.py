@@ -245,6 +245,19 @@ def test_refusals_come_before_anything_is_queued(decoder):
     consistent(dec, {0: 128, 1: 64})
 
 
+def test_token_ids_outside_the_vocabulary_are_refused(decoder):
+    """(On the device an id would be clamped and, as a token to be scored, have a log probability of 0.)"""
+    dec, dev = decoder
+    dev.fail = {name: 0 for name in ("upload", "rbn_kv_plan", "download")}
+    for ids in ([5, 100], [-1], [3, 2 ** 31 + 5], np.array([1, 2 ** 32], np.int64), np.array([2 ** 63 + 1], np.uint64), [1.0, float("nan")]):
+        for call in (dec.start, dec.score):
+            with pytest.raises(ValueError, match="outside"):
+                call({0: [1, 2], 1: ids})
+    dev.fail = {}
+    consistent(dec, {})
+    dec.score({0: [0, 99], 1: [99]})
+
+
 def test_a_device_that_is_gone(decoder):
     """Where not even the lengths can be read back, nothing that follows is done on a guess."""
     dec, dev = decoder
