@@ -134,7 +134,9 @@ static int create_context(int device, bool adopt, hipStream_t stream, rbn_ctx **
         (e = hipMalloc((void **)&ctx->attention_tickets, 2 * RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMemset(ctx->attention_tickets, 0, 2 * RBN_ATTENTION_ITEMS * sizeof(unsigned))) != hipSuccess ||
         (e = hipMalloc((void **)&ctx->dev_flags, 256)) != hipSuccess ||
-        (e = hipMemset(ctx->dev_flags, 0, 256)) != hipSuccess) {
+        (e = hipMemset(ctx->dev_flags, 0, 256)) != hipSuccess ||
+        // the fills are on the default stream, which the context's own does not wait for
+        (e = hipStreamSynchronize(nullptr)) != hipSuccess) {
         int rc = rbn_fail(RBN_ERR_HIP, "context set-up failed: %s", hipGetErrorString(e));
         rbn_ctx_destroy(ctx);
         return rc;
