@@ -91,7 +91,9 @@ int rbn_ctx_create(int device, rbn_ctx **out);
  * every call of the context is ordered with what the caller queues there itself, so memory that
  * another library fills on that stream needs no synchronisation in between.  The stream must
  * belong to `device` and outlive the context, which never destroys it.  Graph capture
- * needs a stream that HIP can capture (not the default one).  No reference counterpart. */
+ * needs a stream that HIP can capture (not the default one).  Captured calls use the context's
+ * workspace like any others: a graph that the caller captured from the stream itself is replayed there, or
+ * ordered with the context's other calls in some other way.  No reference counterpart. */
 int rbn_ctx_create_on_stream(int device, void *stream, rbn_ctx **out);
 int rbn_ctx_destroy(rbn_ctx *ctx);
 int rbn_get_device_info(rbn_ctx *ctx, rbn_device_info *out);

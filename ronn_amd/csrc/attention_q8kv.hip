@@ -316,10 +316,10 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
 //    workgroups that share it.  How many share is decided on the device, where the lengths are: a share is
 //    what gives kTargetGroups shares in all, so that rows of any mix of lengths fill the chip evenly.
 //    The last workgroup of an item to finish joins the partial results in a fixed order.
-// Bound by the reading of the codes where there are many: 64 ragged rows up to 30000, 8 K/V heads, 377 MB: 71 us, 5.3 TB/s, 6.6
-// between start and join (non-temporal loads; 82 with ordinary ones); one row of 131000: 50.5 us.  With few by round trips: 1 row of
+// Bound by the reading of the codes where there are many: 64 ragged rows up to 30000, 8 K/V heads, 377 MB: 71.5 us, 5.3 TB/s, 6.6
+// between start and join (non-temporal loads; 82 with ordinary ones); one row of 131000: 50.6 us.  With few by round trips: 1 row of
 // 1000, 20 heads: 10.3 us (task 2, q and pages 2.7, two blocks 2.7, publishing 1.8, joining 2.5).  A second block on its way per
-// wave changes nothing (71.6, 51.6, 10.6 us): a wave has some 1700 cycles of vector work per block.
+// wave changed nothing (71.6, 51.6, 10.6 us): a wave has some 1800 cycles of vector work per block.
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
 // Blocks a workgroup takes at least before another shares the item: 8 while that gives no more than a
@@ -760,7 +760,7 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
 //    weights cannot have a scale of their own as they have above.)
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 // Bound by the matrix instructions where there is much to do: five prompts of 268 to 1248 behind up to 1631 positions, 20 / 5 heads:
-// 59 us, 343 TFLOP/s (686 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
+// 59.5 us, 341 TFLOP/s (682 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
 // of the SIMD's two waves.  One prompt of 512, 20 heads: 24.3 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
 constexpr int kPromptThreads = 256;
 // Powers of two that the running maximum may lag behind, and log2 of what P is scaled up by.  A lag moves the output less often (five

@@ -340,7 +340,8 @@ class BatchDecoder:
     running row by its greedy token, finish() frees rows.  score() gives the log probabilities of given tokens.
     pages: pages of 32 positions shared by the rows (0: enough for every row at cfg.max_seq); max_tokens: the most
     tokens of one call; top: alternatives that come with every token (1 to 32).  A call that is refused changes nothing; where one
-    fails on the way (a launch, say), the rows that it had advanced on the device end and are free again."""
+    fails on the way (a launch, say), the rows that it had advanced on the device end and are free again.  The decoder does not look at
+    ctx.device_flags(): FLAG_KV_NONFINITE there says that since it was read last a key or value was saturated or a NaN made 0."""
 
     LOGIT_ROWS = 256    # rows of logits computed at a time when prompts are scored
 
