@@ -505,8 +505,9 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
                 for (int d = 0; d < DT; ++d) o[ct][d] *= corr;
             }
             // the block's weights on a scale of their own, the largest in [2^14, 2^15), and that scale in units of the output
+            // (scores beyond 2^24 have no bits left to take 14 off)
             const bool none = m == -INFINITY;
-            const float unit = none ? 0.0f : m - 14.0f;
+            const float unit = none ? 0.0f : m - (fabsf(m) < 16777216.0f ? 14.0f : 0.0f);
             const float up = none ? 0.0f : __builtin_amdgcn_exp2f(unit - run_max[ct]);
             float sum = 0.0f;
 #pragma unroll
@@ -941,6 +942,7 @@ __device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int blo
     }
 
     float run_max = -INFINITY, run_sum = 0.0f;
+    float limit = -INFINITY;  // the running maximum follows scores above this
     int vexp = -200;  // exponent of the output's unit; none yet
     v16f o[NT];
 #pragma unroll
@@ -990,7 +992,8 @@ __device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int blo
             m = max_of(s);
         }
         m *= f;
-        if (__any(m > run_max + (float)kLag)) {
+        bool apart = false;  // the maximum is off the scores already
+        if (__any(m > limit)) {
             m = fmaxf(m, __shfl_xor(m, 32));
             const float mx = fmaxf(run_max, m);
             const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
@@ -1000,10 +1003,19 @@ __device__ __forceinline__ void attend_prompts(PromptShared<HD> &shared, int blo
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[nt][r] *= corr;
+            const float ref = run_max == -INFINITY ? 0.0f : run_max;
+            apart = __any(fabsf(ref) > 1048576.0f);
+            limit = apart ? -INFINITY : run_max + (float)kLag;
+            if (apart) {
+                // with so large a maximum the bias would have too few bits left: it comes off the scores first, in every block
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = s[r] * f - ref;
+                f = 1.0f;
+            }
         }
         // (a block of V's that is all zero: any shift will do)
         const int shift = x.ve != kNone ? kShift - vexp : 0;
-        bias = x.vlog + (float)shift - (run_max == -INFINITY ? 0.0f : run_max);
+        bias = x.vlog + (float)shift - (run_max == -INFINITY || apart ? 0.0f : run_max);
         inverse = ldexpf(x.vinv, -shift);
     };
     // P of the raw scores r and r + 1 as f16 hi + lo; returns their sum.

@@ -16,6 +16,7 @@ import pytest
 
 import batch_model as BM
 from ronn_amd.kvcache import PagedKVCache
+from test_gpu_batch import Rig
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,32 @@ def test_small_weights_of_a_few_tokens(ctx, kv_heads, group, hd, fmt, held, new,
 @pytest.mark.parametrize("late", [False, True])
 def test_small_weights_of_a_prompt(ctx, kv_heads, group, hd, fmt, held, new, peak_v, spread, late):
     check_peaked(ctx, kv_heads, group, hd, fmt, held, new, 64, 50, held - 100 if late else 0, peak_v, spread, True)
+
+
+@pytest.mark.parametrize("hd,fmt", [(64, "i8"), (128, "e4m3")])
+@pytest.mark.parametrize("new,hint", [([1, 1], 1), ([3, 2], 3), ([40, 33], 40)])
+def test_scores_whose_units_are_coarse(ctx, hd, fmt, new, hint):
+    """Scores from 1e5 to 1e36, where f32 has no bits left for a power of two to be taken off: every output is finite, and where the
+    largest score stands clear of the others by more than they can be off, (hd + 8) u sum|q k| / sqrt(hd) each, it is V of that key."""
+    rig = Rig(ctx, 4, 2, hd, fmt, rows=2, max_tokens=512, seed=hd)
+    rig.step([300, 130])
+    q = rig.step(new)
+    k, v = zip(*(rig.device_values(r) for r in range(2)))
+    clear = 0
+    for factor in (1e5, 3e6, 2e7, 1e8, 7e8, 1e10, 1e13, 1e20, 1e35):
+        big = (q * np.float32(factor)).astype(np.float32)
+        rig.d_q.upload(big)
+        out = rig.attend(big, hint)
+        assert np.isfinite(out).all(), factor
+        for i in range(len(q)):
+            r, n = rig.token_row[i], rig.token_pos[i] + 1
+            for h in range(4):
+                kh, vh = k[r][:n, h // 2], v[r][:n, h // 2]
+                s = kh @ big[i, h].astype(np.float64) / np.sqrt(hd)
+                off = (hd + 8) * U * (np.abs(kh) @ np.abs(big[i, h]).astype(np.float64)).max() / np.sqrt(hd)
+                best = int(s.argmax())
+                # 32 below the largest by then, all others together weigh less than n e^-32
+                if s[best] - np.partition(s, -2)[-2] > 2 * off + 32:
+                    clear += 1
+                    assert np.abs(out[i, h] - vh[best]).max() <= 8 * U * np.abs(vh).max() + n * np.exp(-32) * 2 * np.abs(vh).max(), (factor, i, h)
+    assert clear > 20 * len(q)
