@@ -317,14 +317,15 @@ __device__ __forceinline__ Task deal(const KvTableArgs &t, const KvBatchArgs &b,
 //    what gives kTargetGroups shares in all, so that rows of any mix of lengths fill the chip evenly.
 //    The last workgroup of an item to finish joins the partial results in a fixed order.
 // Bound by the reading of the codes where there are many: 64 ragged rows up to 30000, 8 K/V heads, 377 MB: 71.5 us, 5.3 TB/s, 6.6
-// between start and join (non-temporal loads; 82 with ordinary ones); one row of 131000: 50.6 us.  With few by round trips: 1 row of
+// between start and join (non-temporal loads; 82 with ordinary ones); one row of 131000: 50.5 us.  With few by round trips: 1 row of
 // 1000, 20 heads: 10.3 us (task 2, q and pages 2.7, two blocks 2.7, publishing 1.8, joining 2.5).  A second block on its way per
 // wave changed nothing (71.6, 51.6, 10.6 us): a wave has some 1800 cycles of vector work per block.
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = kTokenWaves * 64;
 // Blocks a workgroup takes at least before another shares the item: 8 while that gives no more than a
 // workgroup per CU, up to twice as many beyond (1 x 1000 tokens, 20 heads: 10.9 us with 8, 12.4 with 16; 16 rows of 500 to
-// 4000, 5 heads: 21.0 us with 8, 17.0 with 16).
+// 4000, 5 heads: 21.0 us with 8, 17.0 with 16).  Half or twice both numbers: 1 x 4000, 8 heads, 12.8 and 12.1 us (11.4 as they
+// are), 16 x 2500, 5 heads, 25.2 and 20.2 (20.8), 8 x 8000, 8 heads, 35.3 and 28.1 (33.3), 1 x 300, 20 heads, 9.6 and 7.3 (9.9).
 constexpr int kMinShare = 8;
 constexpr int kTargetGroups = 1536;   // workgroups that share the batch's blocks evenly
 constexpr int kMaxShares = 64;        // one lane for each when they are joined; more cost more there than they gain
@@ -761,15 +762,18 @@ __device__ __forceinline__ void attend_task(TokenShared<HD, NT> &shared, Deal de
 //    weights cannot have a scale of their own as they have above.)
 //  * Every block before a wave's own is full and unmasked, its own is masked, later ones are skipped.
 // Bound by the matrix instructions where there is much to do: five prompts of 268 to 1248 behind up to 1631 positions, 20 / 5 heads:
-// 59.5 us, 341 TFLOP/s (682 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
-// of the SIMD's two waves.  One prompt of 512, 20 heads: 24.3 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
+// 59 us, 345 TFLOP/s (690 with the lo parts); 2750 cycles for a block of a workgroup in the loop, 2110 of them matrix instructions
+// of the SIMD's two waves.  One prompt of 512, 20 heads: 24.7 us, latency (task 4, q, pages and first codes 5, blocks 10, join 5).
 constexpr int kPromptThreads = 256;
 // Powers of two that the running maximum may lag behind, and log2 of what P is scaled up by.  A lag moves the output less often (five
 // ragged prompts: 59.6 us with 8, 60.4 with 4, 60.9 with 3) and leaves P as many bits less.
 constexpr int kLag = 4, kShift = 13 - kLag;
-constexpr int kPromptTargetGroups = 288;  // shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288)
+// Shares in all (five ragged prompts: 61.4 us with 256, 59.7 with 288; the same with either: 5 x 700 behind 900 positions, 20 / 5
+// heads, 116 us, 8 x 300 behind 500, 20 heads, 57, 2 x 1500 behind 1000, 32 / 8 heads, 184).
+constexpr int kPromptTargetGroups = 288;
 // blocks a workgroup takes at least before another shares the tile: partial results cost some 10 us to write, wait for
-// and join, a block 0.75 (one prompt of 512, 20 heads: 27.2 us with 4, 25.5 with 8, 24.7 with 12, 27.9 with 16 or none shared)
+// and join, a block 0.75 (one prompt of 512, 20 heads: 27.2 us with 4, 25.5 with 8, 24.7 with 12, 27.9 with 16 or none shared;
+// 512, 20 / 5 heads: 24.1 with 8 and 12, 27.1 with 16; 1000, 20 heads: 42.5 with 8 and 12, 36.2 with 16)
 constexpr int kPromptMinShare = 12;
 constexpr int kPromptMaxShares = 16;
 
